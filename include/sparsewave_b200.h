@@ -288,6 +288,95 @@ SWB_API int swb_bsr16_spmm_bf16_static(int64_t rows, int64_t cols, int64_t nnzb,
  * on the same device overwrites the record, so ask before making one. */
 SWB_API int swb_bsr16_static_status(swb_stream stream, int32_t *gave_up_ctas);
 
+/* ---- products grouped by expert, 8-bit operands with block scales -------- */
+/* The block-diagonal companion of the BSR product, with ragged blocks: a
+ * mixture-of-experts layer, whose rows (tokens) come sorted by expert.  Not
+ * reference operators. */
+typedef enum swb_dtype {
+  SWB_BF16 = 0,
+  SWB_F16 = 1,
+  SWB_F32 = 2,
+  SWB_E4M3 = 3, /* 8 bits: finite up to 448                                 */
+  SWB_E5M2 = 4  /* 8 bits: finite up to 57344                               */
+} swb_dtype;
+
+/* C[r, :] = A[r, :] B[g] for offsets[g] <= r < offsets[g + 1].
+ *   A        rows x inner, row-major;
+ *   B        groups x inner x n, or groups x n x inner with transpose_b;
+ *   C        rows x n;  offsets: groups + 1 entries on the device.
+ * `dtype` (SWB_BF16 or SWB_F16) is that of A, B and C; sums are f32, rounded
+ * once.  Offsets must not decrease; rows of no group (before offsets[0], from
+ * offsets[groups] on) are neither read nor written, so that a batch may be
+ * padded.  The offsets stay on the device and are read by the kernel: a call
+ * can be captured in a CUDA graph and replayed with other group sizes.  They
+ * are clipped to [0, rows], so that wrong ones make wrong rows and no access
+ * outside the operands.  A group may be empty; inner == 0 makes zeros.  At
+ * most 1024 groups (SWB_ERR_CAPACITY).  A row of C does not depend on the
+ * values in other rows of A, whatever they hold. */
+SWB_API int swb_grouped_mm(swb_context *ctx, int32_t dtype, int64_t rows,
+                           int64_t inner, int64_t n, int64_t groups,
+                           const int32_t *offsets, const void *A, const void *B,
+                           int32_t transpose_b, void *C, swb_stream stream);
+
+/* Gradients of swb_grouped_mm, given dC (rows x n, the operands' type):
+ *   dA[r, :] = dC[r, :] B[g]^T;  rows of no group are left as they were;
+ *   dB[g] = sum over the rows r of group g of A[r, :]^T dC[r, :], in B's
+ *   layout; zeros for an empty group.
+ * dA or dB may be NULL: it is not computed, and what only it needs (B, A) may
+ * be NULL too.  Sums are f32, rounded once, in an order that no launch
+ * changes. */
+SWB_API int swb_grouped_mm_grad(swb_context *ctx, int32_t dtype, int64_t rows,
+                                int64_t inner, int64_t n, int64_t groups,
+                                const int32_t *offsets, const void *A,
+                                const void *B, const void *dC,
+                                int32_t transpose_b, void *dA, void *dB,
+                                swb_stream stream);
+
+/* 8-bit values with a scale for each block of 128: q = x / scale rounded to
+ * fp8_dtype (SWB_E4M3 or SWB_E5M2), scale = max |x| of the block / the largest
+ * value of fp8_dtype, at least 2^-126.  `dtype` is that of X: SWB_BF16,
+ * SWB_F16 or SWB_F32.  A block with a NaN or an infinity gets that as its
+ * scale, and every product with it is NaN.
+ *
+ * Rows (activations): a scale for each 128 columns of a row.  X and Q are
+ * rows x cols, scales is ceil(cols / 128) x rows. */
+SWB_API int swb_fp8_quantize_rows(swb_context *ctx, int32_t dtype,
+                                  int32_t fp8_dtype, int64_t rows, int64_t cols,
+                                  const void *X, void *Q, float *scales,
+                                  swb_stream stream);
+/* Blocks (weights): a scale for each 128 x 128 block.  X and Q are groups x
+ * rows x cols, scales is groups x ceil(rows / 128) x ceil(cols / 128). */
+SWB_API int swb_fp8_quantize_blocks(swb_context *ctx, int32_t dtype,
+                                    int32_t fp8_dtype, int64_t groups,
+                                    int64_t rows, int64_t cols, const void *X,
+                                    void *Q, float *scales, swb_stream stream);
+
+/* C = A B on 8-bit operands: C[r, j] = sum over blocks b of 128 inner elements
+ * of a_scales[b, r] * b_scales[b, j / 128] * sum_{k in b} A[r, k] B[k, j].
+ *   A        rows x inner with the scales of swb_fp8_quantize_rows;
+ *   B        inner x n, or n x inner with transpose_b, with the scales of
+ *            swb_fp8_quantize_blocks on that matrix;
+ *   C        rows x n, bf16.
+ * a_dtype and b_dtype are SWB_E4M3 or SWB_E5M2 each.  Both the sum of a block
+ * and the sum of the scaled blocks are f32.  The gradient with respect to A is
+ * the same call on dC quantised by rows and the same B with the other
+ * transpose_b; the gradient with respect to B is swb_grouped_mm_grad's on the
+ * 16-bit A and dC (8-bit A has its scales along the wrong axis). */
+SWB_API int swb_fp8_mm(swb_context *ctx, int32_t a_dtype, int32_t b_dtype,
+                       int64_t rows, int64_t inner, int64_t n, const void *A,
+                       const float *a_scales, const void *B,
+                       const float *b_scales, int32_t transpose_b, uint16_t *C,
+                       swb_stream stream);
+/* The same grouped by expert as in swb_grouped_mm: B and b_scales have one
+ * more axis of `groups` in front. */
+SWB_API int swb_fp8_grouped_mm(swb_context *ctx, int32_t a_dtype,
+                               int32_t b_dtype, int64_t rows, int64_t inner,
+                               int64_t n, int64_t groups,
+                               const int32_t *offsets, const void *A,
+                               const float *a_scales, const void *B,
+                               const float *b_scales, int32_t transpose_b,
+                               uint16_t *C, swb_stream stream);
+
 /* ---- operators, host buffers ------------------------------------------- */
 /* Same contracts with HOST pointers: the call copies the operands to the
  * context's device workspace (grown on demand and kept), runs the kernel,

@@ -23,6 +23,8 @@ SWB_ERR_UNSUPPORTED = -5
 SWB_ERR_INVALID_DATA = -6
 SWB_ERR_CAPACITY = -7
 
+SWB_BF16, SWB_F16, SWB_F32, SWB_E4M3, SWB_E5M2 = range(5)  # swb_dtype
+
 
 class SwbOptions(C.Structure):
     _fields_ = [
@@ -64,6 +66,7 @@ class Memref2D(C.Structure):
 
 _P = C.c_void_p
 _I64 = C.c_int64
+_I32 = C.c_int32
 _CTX = C.c_void_p
 _OPT = C.POINTER(SwbOptions)
 
@@ -85,6 +88,12 @@ SIGNATURES = {
     "swb_bsr_spmm_bf16": (C.c_int, [_CTX, _OPT, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P]),
     "swb_bsr16_spmm_bf16_static": (C.c_int, [_I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, C.POINTER(C.c_int32)]),
     "swb_bsr16_static_status": (C.c_int, [_P, C.POINTER(C.c_int32)]),
+    "swb_grouped_mm": (C.c_int, [_CTX, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _I32, _P, _P]),
+    "swb_grouped_mm_grad": (C.c_int, [_CTX, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I32, _P, _P, _P]),
+    "swb_fp8_quantize_rows": (C.c_int, [_CTX, _I32, _I32, _I64, _I64, _P, _P, _P, _P]),
+    "swb_fp8_quantize_blocks": (C.c_int, [_CTX, _I32, _I32, _I64, _I64, _I64, _P, _P, _P, _P]),
+    "swb_fp8_mm": (C.c_int, [_CTX, _I32, _I32, _I64, _I64, _I64, _P, _P, _P, _P, _I32, _P, _P]),
+    "swb_fp8_grouped_mm": (C.c_int, [_CTX, _I32, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I32, _P, _P]),
     "swb_spmv_host": (C.c_int, [_CTX, _OPT, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
     "swb_spmm_host": (C.c_int, [_CTX, _OPT, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
     "swb_bsr_spmm_bf16_host": (C.c_int, [_CTX, _OPT, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P]),

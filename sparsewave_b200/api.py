@@ -285,6 +285,43 @@ class Context:
         return self._fast.bsr_spmm(self._ctx.value, self.device, options, block_row_ptr, block_col_idx, block_values, B,
                                    block_size, C_out)
 
+    # -- products grouped by expert, 8-bit operands (device tensors) -----------------
+    def grouped_mm(self, offsets, A, B, C_out=None, *, transpose_b: bool = False):
+        """C[r] = A[r] @ B[g] for offsets[g] <= r < offsets[g + 1]: the layer of experts whose rows come sorted by
+        expert.  bf16 or f16; A is rows x inner, B groups x inner x n (groups x n x inner with `transpose_b`), offsets
+        groups + 1 int32 on the device, which no call copies to the host.  Rows of no group are left as they were
+        (unset in a C that the call allocates)."""
+        return self._fast.grouped_mm(self._ctx.value, self.device, offsets, A, B, C_out, transpose_b)
+
+    def grouped_mm_grad(self, offsets, A, B, dC, dA=None, dB=None, *, transpose_b: bool = False, need_dA: bool = True,
+                        need_dB: bool = True):
+        """(dA, dB) of `grouped_mm` for the gradient dC of its result; None for one that is not needed.  dB is zero for a
+        group without rows; rows of dA of no group are left as they were."""
+        return self._fast.grouped_mm_grad(self._ctx.value, self.device, offsets, A, B, dC, dA, dB, transpose_b, need_dA,
+                                          need_dB)
+
+    def fp8_quantize_rows(self, X, Q=None, scales=None, *, dtype=torch.float8_e4m3fn):
+        """X (rows x cols; bf16, f16 or f32) as 8-bit values with a scale for each 128 columns of a row: (Q, scales),
+        scales f32, ceil(cols / 128) x rows."""
+        return self._fast.fp8_quantize(self._ctx.value, self.device, True, X, Q, scales, dtype)
+
+    def fp8_quantize_blocks(self, X, Q=None, scales=None, *, dtype=torch.float8_e4m3fn):
+        """X (a matrix or a stack of matrices) as 8-bit values with a scale for each block of 128 x 128: (Q, scales),
+        scales f32, [groups x] ceil(rows / 128) x ceil(cols / 128)."""
+        return self._fast.fp8_quantize(self._ctx.value, self.device, False, X, Q, scales, dtype)
+
+    def fp8_mm(self, A, a_scales, B, b_scales, C_out=None, *, transpose_b: bool = False):
+        """C = A @ B (A @ B.T with `transpose_b`) in bf16 for A from `fp8_quantize_rows` and B from
+        `fp8_quantize_blocks`, with f32 sums.  The gradient of A is the same call on the quantised dC with the other
+        `transpose_b`; that of B `grouped_mm_grad`'s on the 16-bit A."""
+        return self._fast.fp8_product(self._ctx.value, self.device, None, A, a_scales, B, b_scales, C_out, transpose_b)
+
+    def fp8_grouped_mm(self, offsets, A, a_scales, B, b_scales, C_out=None, *, transpose_b: bool = False):
+        """`fp8_mm` grouped by expert as in `grouped_mm`: B and b_scales have one more axis of groups in front."""
+        if offsets is None:
+            raise TypeError("offsets must be a CUDA tensor")
+        return self._fast.fp8_product(self._ctx.value, self.device, offsets, A, a_scales, B, b_scales, C_out, transpose_b)
+
     def bundle_launch(self, operation: str, n: int, args) -> None:
         """lrrt-style launch: five device pointers (rowOffsets, columnIndices, values, rhs, output)."""
         arr = (C.c_void_p * 5)(*[a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args])

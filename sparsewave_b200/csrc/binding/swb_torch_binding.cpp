@@ -9,11 +9,13 @@
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <string>
 #include <unordered_map>
+#include <vector>
 
 #include "../../../include/sparsewave_b200.h"
 
@@ -248,6 +250,217 @@ PyObject *bsr_spmm(PyObject *, PyObject *const *a, Py_ssize_t n) {
   });
 }
 
+// ---- products grouped by expert, 8-bit operands ------------------------------------------------------------------------
+
+[[noreturn]] void raise_shape(const std::string &message) { raise_status(SWB_ERR_INVALID_SHAPE, message.c_str()); }
+
+// A tensor of `rank` dimensions on the context's device.
+const at::Tensor &operand(PyObject *obj, int64_t rank, int64_t device, const char *name) {
+  const at::Tensor &t = tensor(obj, name);
+  if (!t.is_cuda()) raise_type(name, "must be a CUDA tensor");
+  if (t.get_device() != device) raise_type(name, "must be on the context's device");
+  if (t.dim() != rank)
+    raise_shape(std::string(name) + " must have " + std::to_string(rank) + " dimensions, but got " + std::to_string(t.dim()));
+  return t;
+}
+
+void require_sizes(const at::Tensor &t, at::IntArrayRef sizes, const char *name) {
+  if (t.sizes() == sizes) return;
+  std::string want, got;
+  for (int64_t s : sizes) want += (want.empty() ? "" : " x ") + std::to_string(s);
+  for (int64_t s : t.sizes()) got += (got.empty() ? "" : " x ") + std::to_string(s);
+  raise_shape(std::string(name) + " must be " + want + ", but got " + got);
+}
+
+enum class Types { k16Bits, k16BitsOrF32, kFp8 };
+
+int type_code(const at::Tensor &t, const char *name, Types allowed) {
+  const bool fp8 = allowed == Types::kFp8;
+  switch (t.scalar_type()) {
+    case at::kBFloat16: if (!fp8) return SWB_BF16; break;
+    case at::kHalf: if (!fp8) return SWB_F16; break;
+    case at::kFloat: if (allowed == Types::k16BitsOrF32) return SWB_F32; break;
+    case at::kFloat8_e4m3fn: if (fp8) return SWB_E4M3; break;
+    case at::kFloat8_e5m2: if (fp8) return SWB_E5M2; break;
+    default: break;
+  }
+  raise_type(name, fp8                           ? "must be float8_e4m3fn or float8_e5m2"
+                   : allowed == Types::k16Bits ? "must be bfloat16 or float16"
+                                                 : "must be bfloat16, float16 or float32");
+}
+
+bool truth(PyObject *obj) {
+  const int t = PyObject_IsTrue(obj);
+  if (t < 0) throw Failed();
+  return t != 0;
+}
+
+// The output that the caller gave, checked, or a fresh one.
+at::Tensor output_of(PyObject *given, at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor &like, int64_t device,
+                     const char *name) {
+  if (given == Py_None) return at::empty(sizes, at::TensorOptions().dtype(dtype).device(like.device()));
+  const at::Tensor &t = operand(given, (int64_t)sizes.size(), device, name);
+  require_sizes(t, sizes, name);
+  device_pointer(t, dtype, name);
+  return t;
+}
+
+template <typename Call>
+void call_library(swb_context *ctx, Call call) {
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = call();
+  Py_END_ALLOW_THREADS
+  if (st != SWB_OK) raise_status(st, swb_last_error(ctx));
+}
+
+PyObject *wrapped(PyObject *given, at::Tensor &t) {
+  if (given != Py_None) {
+    Py_INCREF(given);
+    return given;
+  }
+  return THPVariable_Wrap(std::move(t));
+}
+
+PyObject *pair(PyObject *first, PyObject *second) {
+  PyObject *both = first && second ? PyTuple_New(2) : nullptr;
+  if (!both) {
+    Py_XDECREF(first);
+    Py_XDECREF(second);
+    throw Failed();
+  }
+  PyTuple_SET_ITEM(both, 0, first);
+  PyTuple_SET_ITEM(both, 1, second);
+  return both;
+}
+
+// grouped_mm(ctx, device, offsets, A, B, C | None, transpose_b)
+PyObject *grouped_mm(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded(n, 7, [&]() -> PyObject * {
+    swb_context *ctx = context_of(a[0]);
+    const int64_t device = integer(a[1]);
+    const at::Tensor &off = operand(a[2], 1, device, "offsets"), &A = operand(a[3], 2, device, "A"),
+                     &B = operand(a[4], 3, device, "B");
+    const bool tb = truth(a[6]);
+    const int64_t rows = A.size(0), inner = A.size(1), groups = B.size(0), cols = B.size(tb ? 1 : 2);
+    require_sizes(off, {groups + 1}, "offsets");
+    require_sizes(B, {groups, tb ? cols : inner, tb ? inner : cols}, "B");
+    const int type = type_code(A, "A", Types::k16Bits);
+    auto *p_off = (const int32_t *)device_pointer(off, at::kInt, "offsets");
+    void *p_A = device_pointer(A, A.scalar_type(), "A"), *p_B = device_pointer(B, A.scalar_type(), "B");
+    at::Tensor C = output_of(a[5], {rows, cols}, A.scalar_type(), A, device, "C");
+    void *s = stream_of(a[1]);
+    call_library(ctx, [&] {
+      return swb_grouped_mm(ctx, type, rows, inner, cols, groups, p_off, p_A, p_B, tb, C.data_ptr(), s);
+    });
+    return wrapped(a[5], C);
+  });
+}
+
+// grouped_mm_grad(ctx, device, offsets, A, B, dC, dA | None, dB | None, transpose_b, need_dA, need_dB)
+PyObject *grouped_mm_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded(n, 11, [&]() -> PyObject * {
+    swb_context *ctx = context_of(a[0]);
+    const int64_t device = integer(a[1]);
+    const at::Tensor &off = operand(a[2], 1, device, "offsets"), &A = operand(a[3], 2, device, "A"),
+                     &B = operand(a[4], 3, device, "B"), &dC = operand(a[5], 2, device, "dC");
+    const bool tb = truth(a[8]), need_a = truth(a[9]), need_b = truth(a[10]);
+    const int64_t rows = A.size(0), inner = A.size(1), groups = B.size(0), cols = dC.size(1);
+    const at::ScalarType dt = A.scalar_type();
+    require_sizes(off, {groups + 1}, "offsets");
+    require_sizes(dC, {rows, cols}, "dC");
+    require_sizes(B, {groups, tb ? cols : inner, tb ? inner : cols}, "B");
+    const int type = type_code(A, "A", Types::k16Bits);
+    auto *p_off = (const int32_t *)device_pointer(off, at::kInt, "offsets");
+    void *p_A = device_pointer(A, dt, "A"), *p_B = device_pointer(B, dt, "B"), *p_dC = device_pointer(dC, dt, "dC");
+    at::Tensor dA, dB;
+    if (need_a) dA = output_of(a[6], A.sizes(), dt, A, device, "dA");
+    if (need_b) dB = output_of(a[7], B.sizes(), dt, A, device, "dB");
+    void *p_dA = need_a ? dA.data_ptr() : nullptr, *p_dB = need_b ? dB.data_ptr() : nullptr, *s = stream_of(a[1]);
+    call_library(ctx, [&] {
+      return swb_grouped_mm_grad(ctx, type, rows, inner, cols, groups, p_off, p_A, p_B, p_dC, tb, p_dA, p_dB, s);
+    });
+    PyObject *first = need_a ? wrapped(a[6], dA) : (Py_INCREF(Py_None), Py_None);
+    PyObject *second = need_b ? wrapped(a[7], dB) : (Py_INCREF(Py_None), Py_None);
+    return pair(first, second);
+  });
+}
+
+at::ScalarType fp8_type(PyObject *obj) {
+  if (THPDtype_Check(obj)) {
+    const at::ScalarType t = reinterpret_cast<THPDtype *>(obj)->scalar_type;
+    if (t == at::kFloat8_e4m3fn || t == at::kFloat8_e5m2) return t;
+  }
+  raise_type("dtype", "must be torch.float8_e4m3fn or torch.float8_e5m2");
+}
+
+// fp8_quantize(ctx, device, by_rows, X, Q | None, scales | None, dtype)
+PyObject *fp8_quantize(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded(n, 7, [&]() -> PyObject * {
+    swb_context *ctx = context_of(a[0]);
+    const int64_t device = integer(a[1]);
+    const bool by_rows = truth(a[2]);
+    const at::Tensor &given = tensor(a[3], "X");
+    const at::Tensor &X = operand(a[3], by_rows || given.dim() == 2 ? 2 : 3, device, "X");
+    const int64_t d = X.dim(), groups = d == 3 ? X.size(0) : 1, rows = X.size(d - 2), cols = X.size(d - 1);
+    const int type = type_code(X, "X", Types::k16BitsOrF32);
+    const at::ScalarType out = fp8_type(a[6]);
+    void *p_X = device_pointer(X, X.scalar_type(), "X");
+    const int64_t rb = (rows + 127) / 128, cb = (cols + 127) / 128;
+    const std::vector<int64_t> sizes = by_rows  ? std::vector<int64_t>{cb, rows}
+                                       : d == 3 ? std::vector<int64_t>{groups, rb, cb}
+                                                : std::vector<int64_t>{rb, cb};
+    at::Tensor Q = output_of(a[4], X.sizes(), out, X, device, "Q"), scales = output_of(a[5], sizes, at::kFloat, X, device, "scales");
+    void *p_Q = Q.data_ptr(), *s = stream_of(a[1]);
+    auto *p_s = (float *)scales.data_ptr();
+    const int fp8 = out == at::kFloat8_e5m2 ? SWB_E5M2 : SWB_E4M3;
+    call_library(ctx, [&] {
+      return by_rows ? swb_fp8_quantize_rows(ctx, type, fp8, rows, cols, p_X, p_Q, p_s, s)
+                     : swb_fp8_quantize_blocks(ctx, type, fp8, groups, rows, cols, p_X, p_Q, p_s, s);
+    });
+    PyObject *first = wrapped(a[4], Q);
+    return pair(first, wrapped(a[5], scales));
+  });
+}
+
+// fp8_product(ctx, device, offsets | None, A, a_scales, B, b_scales, C | None, transpose_b): without offsets B is one matrix
+PyObject *fp8_product(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject * {
+    swb_context *ctx = context_of(a[0]);
+    const int64_t device = integer(a[1]);
+    const bool grouped = a[2] != Py_None, tb = truth(a[8]);
+    const int64_t front = grouped ? 1 : 0;
+    const at::Tensor &A = operand(a[3], 2, device, "A"), &as = operand(a[4], 2, device, "a_scales"),
+                     &B = operand(a[5], 2 + front, device, "B"), &bs = operand(a[6], 2 + front, device, "b_scales");
+    const int64_t rows = A.size(0), inner = A.size(1), groups = grouped ? B.size(0) : 1, cols = B.size(front + (tb ? 0 : 1));
+    const int64_t kb = (inner + 127) / 128, nb = (cols + 127) / 128;
+    std::vector<int64_t> b_sizes{tb ? cols : inner, tb ? inner : cols}, s_sizes{tb ? nb : kb, tb ? kb : nb};
+    const int32_t *p_off = nullptr;
+    if (grouped) {
+      const at::Tensor &off = operand(a[2], 1, device, "offsets");
+      require_sizes(off, {groups + 1}, "offsets");
+      p_off = (const int32_t *)device_pointer(off, at::kInt, "offsets");
+      b_sizes.insert(b_sizes.begin(), groups);
+      s_sizes.insert(s_sizes.begin(), groups);
+    }
+    require_sizes(B, b_sizes, "B");
+    require_sizes(as, {kb, rows}, "a_scales");
+    require_sizes(bs, s_sizes, "b_scales");
+    const int a_type = type_code(A, "A", Types::kFp8), b_type = type_code(B, "B", Types::kFp8);
+    void *p_A = device_pointer(A, A.scalar_type(), "A"), *p_B = device_pointer(B, B.scalar_type(), "B");
+    auto *p_as = (const float *)device_pointer(as, at::kFloat, "a_scales");
+    auto *p_bs = (const float *)device_pointer(bs, at::kFloat, "b_scales");
+    at::Tensor C = output_of(a[7], {rows, cols}, at::kBFloat16, A, device, "C");
+    auto *p_C = (uint16_t *)C.data_ptr();
+    void *s = stream_of(a[1]);
+    call_library(ctx, [&] {
+      return grouped ? swb_fp8_grouped_mm(ctx, a_type, b_type, rows, inner, cols, groups, p_off, p_A, p_as, p_B, p_bs, tb, p_C, s)
+                     : swb_fp8_mm(ctx, a_type, b_type, rows, inner, cols, p_A, p_as, p_B, p_bs, tb, p_C, s);
+    });
+    return wrapped(a[7], C);
+  });
+}
+
 // bind(SparseWaveError, SwbOptions): the Python types that the calls above raise and accept
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return guarded(n, 2, [&]() -> PyObject * {
@@ -261,7 +474,8 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
 }
 
 #define SWB_FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef g_methods[] = {SWB_FAST(spmv), SWB_FAST(coo_spmv), SWB_FAST(spmm), SWB_FAST(bsr_spmm), SWB_FAST(bind),
+PyMethodDef g_methods[] = {SWB_FAST(spmv), SWB_FAST(coo_spmv), SWB_FAST(spmm), SWB_FAST(bsr_spmm), SWB_FAST(grouped_mm),
+                           SWB_FAST(grouped_mm_grad), SWB_FAST(fp8_quantize), SWB_FAST(fp8_product), SWB_FAST(bind),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "swb_torch", "Device-tensor operator calls over the C ABI.", -1, g_methods,
                         nullptr, nullptr, nullptr, nullptr};

@@ -85,6 +85,8 @@ bool context_comm_shape(const swb_context *ctx, int *n_ranks, int *rank) {
 void *context_peer_window(const swb_context *ctx) { return ctx->peer_window; }
 void set_context_peer_window(swb_context *ctx, void *window) { ctx->peer_window = window; }
 int *context_status_flag(const swb_context *ctx) { return ctx->status_flag; }
+const DeviceInfo &context_device_info(const swb_context *ctx) { return ctx->dev; }
+int64_t *context_launches(swb_context *ctx) { return &ctx->launches; }
 void count_launch(swb_context *ctx) { ++ctx->launches; }
 }  // namespace swb
 

@@ -41,6 +41,39 @@ struct BsrSpmmArgs {
   void *C;
 };
 
+// Element types (swb_dtype of sparsewave_b200.h).
+enum ElementType : int { kBF16 = 0, kF16 = 1, kF32 = 2, kE4M3 = 3, kE5M2 = 4 };
+constexpr int64_t kMaxGroups = 1024;
+constexpr int64_t kScaleBlock = 128;  // elements along an axis that share a scale
+
+// C[r, :] = A[r, :] B[g] for the rows r of group g; `type` kBF16 or kF16, or 8-bit operands with scales and C in bf16.
+struct GroupedArgs {
+  int64_t rows, inner, n, groups;
+  const int32_t *offsets;  // groups + 1; NULL: one group of all rows
+  const void *A, *B;       // rows x inner; groups x inner x n, or n x inner with transpose_b
+  bool transpose_b;
+  void *C;
+  int type;
+  int b_type = 0;  // of 8-bit operands
+  const float *a_scales = nullptr, *b_scales = nullptr;
+};
+// out[g][i, j] = sum over the rows r of group g of left[r, i] * right[r, j]; `type` kBF16 or kF16.
+struct GroupedInnerArgs {
+  int64_t rows, i_size, j_size, groups;
+  const int32_t *offsets;
+  const void *left, *right;
+  void *out;
+  int type;
+};
+// Blocks of X that share a scale: `block_rows` (1 or 128) x 128 elements of each of `groups` matrices.
+struct QuantizeArgs {
+  int64_t groups, rows, cols;
+  const void *X;
+  void *Q;
+  float *scales;  // block_rows 1: (column blocks) x rows; 128: groups x (row blocks) x (column blocks)
+  int type, fp8_type;
+};
+
 // Optional per-position trace of a position-mapped SpMV (all nnz entries).
 struct PositionTrace {
   int32_t *row_of_position = nullptr;
@@ -145,6 +178,12 @@ bool bsr_tcgen05_pays(const BsrSpmmArgs &a, int sm_count);  // and supported; fa
 cudaError_t launch_bsr_spmm_tcgen05(const BsrSpmmArgs &a, int *status_flag, const DeviceInfo &dev, cudaStream_t s,
                                     int64_t *launches);
 
+// --- products grouped by expert, 8-bit operands
+cudaError_t launch_grouped_rows_general(const GroupedArgs &a, cudaStream_t s, int64_t *launches);
+cudaError_t launch_grouped_inner_general(const GroupedInnerArgs &a, cudaStream_t s, int64_t *launches);
+cudaError_t launch_quantize_rows(const QuantizeArgs &a, cudaStream_t s, int64_t *launches);
+cudaError_t launch_quantize_blocks(const QuantizeArgs &a, cudaStream_t s, int64_t *launches);
+
 // Context accessors for translation units that do not see the context's layout.
 }  // namespace swb
 struct swb_context;
@@ -162,6 +201,8 @@ int window_allgather_and_fill(swb_context *ctx, const void *send, float *zero, i
                               bool alternate, const void **gathered);
 void abandon_peer_window(swb_context *ctx);  // non-collective tear-down (swb_peer_window.cu)
 int *context_status_flag(const swb_context *ctx);
+const DeviceInfo &context_device_info(const swb_context *ctx);
+int64_t *context_launches(swb_context *ctx);
 void count_launch(swb_context *ctx);
 
 // Stores the diagnostic that swb_last_error(NULL) returns on this thread.
