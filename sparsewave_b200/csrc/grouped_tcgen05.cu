@@ -1,0 +1,809 @@
+// Products grouped by expert on the Blackwell tensor cores: TMA -> shared memory -> tcgen05.mma -> TMEM -> tcgen05.ld.
+//   rows:  C[r, j] = sum_k A[r, k] B[g][k, j]            r in group g; bf16, fp16, or 8 bits with block scales
+//   inner: D[g][i, j] = sum over r in group g of L[r, i] R[r, j]   (the gradient of the weights)
+//
+// The product is formed transposed.  The 128 lanes of an accumulator (M of the MMA) are output columns j, which are adjacent in
+// memory, so that a warp's store is one run of them; the accumulator's columns (N of the MMA) are rows of the group, and N is
+// chosen tile by tile in steps of 16: a group of 20 rows costs 32, not the 128 that rows on the M side would cost.
+//
+// Tiles.  Wide: pairs of CTAs (cta_group::2) make 256 output columns x up to 256 rows; each CTA loads its 128 columns of the
+// weights and half of the rows, so that an operand byte feeds twice the work that it feeds in one CTA.  Narrow, for groups of few
+// rows, whose time is the reading of the weights: one CTA makes 128 columns x up to 64 rows, and a cluster of up to eight CTAs
+// shares the inner axis of a tile where there are few tiles; their sums are added through distributed shared memory, in the order
+// of the CTAs' ranks, so that results do not depend on timing and no workspace is needed.
+//
+// Which tile lies where is worked out on the device from the offsets: every CTA builds the table of the groups' tiles in shared
+// memory, and the CTAs (pairs, clusters) walk the tiles in turn.
+//
+// Roles: lane 0 of warp 0 copies, lane 0 of warp 1 issues the MMAs, warp 2 clears the rows behind a group's last (inner form),
+// four warps (wide 8-bit: eight) from warp 4 on read the accumulators, round and store.
+//
+// 8-bit operands: the 128 products of a scale block are one chain of the tensor core in an accumulator of its own; the storing
+// warps add it, times the scales of its row and block, to f32 sums in their registers (two sums per fma.f32x2).
+//
+// Every mbarrier wait is bounded: when one runs out the kernel raises the status word, frees its TMEM columns and returns.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <atomic>
+
+#include "grouped_tiles.cuh"
+#include "swb_chain.cuh"
+#include "swb_index.h"
+#include "swb_kernels.h"
+
+namespace swb {
+namespace {
+
+constexpr uint32_t WAIT_LIMIT = 1u << 24;
+constexpr int LANES = 128;           // output columns of a CTA's tile
+constexpr int ROW_BYTES = 128;       // of a swizzled row of an operand in shared memory
+constexpr int BOX_BYTES = 64 * ROW_BYTES;  // a box of 64 inner rows x 64 16-bit elements
+constexpr int FIRST_STORE_WARP = 4;
+constexpr unsigned FULL = 0xffffffffu;
+
+template <int CTAS_, int TILE_, bool FP8_, bool MN_, bool INNER_>
+struct Config {
+  static constexpr int CTAS = CTAS_, TILE = TILE_;   // TILE: accumulator columns, the rows of a tile
+  static constexpr bool FP8 = FP8_, MN = MN_, INNER = INNER_;  // MN: the lanes' operand has its columns contiguous
+  static constexpr int STEP = FP8 ? 128 : 64;        // inner elements of a stage: 128 bytes
+  static constexpr int MMA_STEP = FP8 ? 32 : 16;     // of an MMA
+  static constexpr int ROWS_CTA = TILE / CTAS;       // of a tile's rows in one CTA's shared memory
+  static constexpr int ROW_BOX = INNER ? 64 : CTAS == 2 ? 32 : 16;  // rows of a copy
+  static constexpr int L_BYTES = LANES * ROW_BYTES, T_BYTES = ROWS_CTA * ROW_BYTES, STAGE = L_BYTES + T_BYTES;
+  static constexpr int BUFFERS = 512 / TILE < 4 ? 512 / TILE : 4;
+  static constexpr int TMEM_COLS = BUFFERS * TILE;
+  static constexpr int STORE_WARPS = FP8 && TILE == 256 ? 8 : 4;
+  static constexpr int WARP_COLS = TILE / (STORE_WARPS / 4);  // accumulator columns of a storing warp
+  static constexpr int THREADS = 32 * (FIRST_STORE_WARP + STORE_WARPS);
+  static constexpr bool SPLITS = CTAS == 1 && !INNER;
+  static constexpr int PARTIAL = SPLITS ? TILE * LANES * 4 : 0;       // f32 sums of this CTA's share of the inner axis
+  static constexpr int SCALES = FP8 ? STORE_WARPS * 2 * WARP_COLS * 4 : 0;
+  static constexpr int TABLE = (int)kMaxGroups * 12 + 16;             // spans and tile counts
+  static constexpr int STAGES = (232448 - 1024 - 512 - PARTIAL - SCALES - TABLE) / STAGE;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + PARTIAL + SCALES + TABLE;
+  static constexpr int ROUND = 16 * CTAS;                             // N of an MMA is a multiple of this
+};
+
+struct Product {
+  int rows, inner, cols, groups;  // inner form: `inner` is the size of i, `cols` that of j
+  const int32_t *offsets;
+  uint16_t *out;
+  uint32_t instruction;           // descriptor without N
+  bool half_out;
+  const float *a_scales, *b_scales;
+  int scale_k, scale_j, scale_group;
+  int *status;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ uint64_t make_desc(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {  // 128-byte swizzle
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo_bytes >> 4) & 0x3FFFu) << 16) |
+         ((uint64_t)((sbo_bytes >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+// `bar` may be another CTA's of the cluster (mapped).
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t mapped(uint32_t addr, uint32_t rank) {  // the same place in CTA `rank` of the cluster
+  uint32_t out;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
+  return out;
+}
+
+template <int CTAS>
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                     dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+
+template <int CTAS, bool FP8>
+__device__ __forceinline__ void issue_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, bool add) {
+#define SWB_MMA(group, kind)                                                                                     \
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma." group "." kind " [%0], %1, %2, %3, p;\n\t}" ::"r"(d), \
+               "l"(a), "l"(b), "r"(instruction), "r"(add ? 1u : 0u) : "memory")
+  if constexpr (CTAS == 2 && FP8) SWB_MMA("cta_group::2", "kind::f8f6f4");
+  else if constexpr (CTAS == 2) SWB_MMA("cta_group::2", "kind::f16");
+  else if constexpr (FP8) SWB_MMA("cta_group::1", "kind::f8f6f4");
+  else SWB_MMA("cta_group::1", "kind::f16");
+#undef SWB_MMA
+}
+// Arrives on `bar` (of both CTAs of a pair) when the MMAs issued so far have completed.
+template <int CTAS>
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  if constexpr (CTAS == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"((uint16_t)3) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// 32 accumulator columns of the warp's 32 lanes.
+__device__ __forceinline__ void tmem_load(uint32_t (&v)[32], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+        "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ uint64_t pack(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack(uint64_t v, uint32_t &lo, uint32_t &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {  // two f32 each
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+__device__ __forceinline__ uint16_t rounded(float v, bool half_out) {  // once, to nearest
+  return half_out ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+
+// Row tiles of a group of m rows: as few as the tile size allows, of equal heights but for the last.
+__device__ __forceinline__ void row_tiles(int m, int tile, int round, int *count, int *height) {
+  *count = (m + tile - 1) / tile;
+  *height = *count ? ((m + *count - 1) / *count + round - 1) / round * round : round;
+}
+
+struct Tile {
+  int group, row0, valid, n;  // rows [row0, row0 + valid) as accumulator columns, n of them computed (inner form: of axis i)
+  int col0;                   // first output column of this CTA (pair)
+  int k0, k_blocks, k_valid;  // first stage of the inner axis, stages, elements of the last that exist
+};
+
+template <class S>
+struct Tiles {
+  const int2 *spans;
+  const int *first;  // first tile of each group, and the end
+  int groups, total, col_tiles, inner_tiles;
+
+  __device__ __forceinline__ Tile at(int t, const Product &p, int part, int parts) const {
+    Tile tile;
+    if constexpr (S::INNER) {
+      const int per_group = col_tiles * inner_tiles;
+      tile.group = t / per_group;
+      const int local = t - tile.group * per_group, it = local % inner_tiles;
+      tile.col0 = local / inner_tiles * (LANES * S::CTAS);
+      tile.row0 = it * S::TILE;
+      tile.valid = p.inner - tile.row0 < S::TILE ? p.inner - tile.row0 : S::TILE;
+      tile.n = (tile.valid + S::ROUND - 1) / S::ROUND * S::ROUND;
+      const int2 span = spans[tile.group];
+      const int m = span.y - span.x;
+      tile.k0 = span.x;
+      tile.k_blocks = (m + S::STEP - 1) / S::STEP;
+      tile.k_valid = m - (tile.k_blocks - 1) * S::STEP;
+    } else {
+      int lo = 0, hi = groups;  // the last group whose first tile is at most t
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (first[mid] <= t) lo = mid; else hi = mid;
+      }
+      tile.group = lo;
+      const int2 span = spans[lo];
+      int count, height;
+      row_tiles(span.y - span.x, S::TILE, S::ROUND, &count, &height);
+      // bands of eight row tiles, column tile after column tile within one: what runs at a time shares both operands in L2
+      const int local = t - first[lo], band = local / (8 * col_tiles), in_band = local - band * 8 * col_tiles;
+      const int band_rows = count - band * 8 < 8 ? count - band * 8 : 8;
+      const int row_tile = band * 8 + in_band % band_rows;
+      tile.col0 = in_band / band_rows * (LANES * S::CTAS);
+      tile.row0 = span.x + row_tile * height;
+      tile.valid = span.y - tile.row0 < height ? span.y - tile.row0 : height;
+      tile.n = (tile.valid + S::ROUND - 1) / S::ROUND * S::ROUND;
+      const int blocks = (p.inner + S::STEP - 1) / S::STEP;
+      tile.k0 = (int)((int64_t)blocks * part / parts);
+      tile.k_blocks = (int)((int64_t)blocks * (part + 1) / parts) - tile.k0;
+      tile.k_valid = S::STEP;  // copies fill what lies behind the axis with zeros
+    }
+    return tile;
+  }
+};
+
+template <class S>
+__global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap map_l,
+                                                                        const __grid_constant__ CUtensorMap map_t, const Product p,
+                                                                        const int parts) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bar_full[S::STAGES], bar_empty[S::STAGES], bar_landed[S::STAGES];
+  __shared__ __align__(8) uint64_t bar_sums[S::BUFFERS], bar_stored[S::BUFFERS], bar_parts, bar_added;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t stage0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t *behind = smem_raw + (stage0 - smem_u32(smem_raw)) + S::STAGES * S::STAGE;
+  float *partial = reinterpret_cast<float *>(behind);                         // [TILE][LANES]
+  float *scales = reinterpret_cast<float *>(behind + S::PARTIAL);             // [warp][2][WARP_COLS]
+  int2 *spans = reinterpret_cast<int2 *>(behind + S::PARTIAL + S::SCALES);
+  int *first = reinterpret_cast<int *>(spans + kMaxGroups);
+  const int rank = S::CTAS == 2 || S::SPLITS ? (int)(blockIdx.x % (unsigned)(S::CTAS == 2 ? 2 : parts)) : 0;
+  const int part = S::CTAS == 2 ? 0 : rank;  // of the inner axis
+  const int walkers = (int)gridDim.x / (S::CTAS == 2 ? 2 : parts), walker = (int)blockIdx.x / (S::CTAS == 2 ? 2 : parts);
+
+  after_previous_kernel();
+  if (tid == 0) {
+    failed = 0;
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(smem_u32(&bar_full[s]), S::CTAS);
+      mbar_init(smem_u32(&bar_empty[s]), 1);
+      mbar_init(smem_u32(&bar_landed[s]), 1);
+    }
+    for (int a = 0; a < S::BUFFERS; ++a) {
+      mbar_init(smem_u32(&bar_sums[a]), 1);
+      mbar_init(smem_u32(&bar_stored[a]), S::STORE_WARPS * S::CTAS);
+    }
+    mbar_init(smem_u32(&bar_parts), S::STORE_WARPS * parts);
+    mbar_init(smem_u32(&bar_added), S::STORE_WARPS * parts);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_l) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_t) : "memory");
+  }
+  if (warp == 1) {
+    if constexpr (S::CTAS == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                   "r"(S::TMEM_COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                   "r"(S::TMEM_COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  }
+  Tiles<S> tiles;
+  tiles.spans = spans;
+  tiles.first = first;
+  tiles.groups = p.groups;
+  tiles.col_tiles = (p.cols + LANES * S::CTAS - 1) / (LANES * S::CTAS);
+  tiles.inner_tiles = (p.inner + S::TILE - 1) / S::TILE;
+  for (int g = tid; g < p.groups; g += S::THREADS) {
+    const RowSpan span = group_rows(p.offsets, g, p.rows);
+    spans[g] = make_int2(span.begin, span.end);
+  }
+  __syncthreads();
+  if constexpr (!S::INNER) {
+    if (warp == 0) {
+      int before = 0;
+      for (int g0 = 0; g0 < p.groups; g0 += 32) {
+        int count = 0, height;
+        if (g0 + lane < p.groups) row_tiles(spans[g0 + lane].y - spans[g0 + lane].x, S::TILE, S::ROUND, &count, &height);
+        int through = count * tiles.col_tiles;
+        const int own = through;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+          const int v = __shfl_up_sync(FULL, through, d);
+          if (lane >= d) through += v;
+        }
+        if (g0 + lane < p.groups) first[g0 + lane] = before + through - own;
+        before += __shfl_sync(FULL, through, 31);
+      }
+      if (lane == 0) first[p.groups] = before;
+    }
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  if (S::CTAS == 2 || parts > 1) {  // barriers of the other CTAs are ready too
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+  tiles.total = S::INNER ? p.groups * tiles.col_tiles * tiles.inner_tiles : first[p.groups];
+
+  auto gave_up = [&] {
+    failed = 1;
+    atomicExch(p.status, 1);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t round = 0;
+      bool ok = true;
+      const uint32_t leader_full = S::CTAS == 2 ? mapped(smem_u32(bar_full), 0) : smem_u32(bar_full);
+      for (int t = walker; ok && t < tiles.total; t += walkers) {
+        const Tile tile = tiles.at(t, p, part, parts);
+        const int mine = tile.n / S::CTAS, row = tile.row0 + (S::CTAS == 2 ? rank * mine : 0);
+        const int col = tile.col0 + (S::CTAS == 2 ? rank * LANES : 0);
+        for (int kb = 0; kb < tile.k_blocks; ++kb) {
+          if (round > 0) ok = mbar_wait(smem_u32(&bar_empty[s]), (round - 1) & 1u);
+          if (!ok) {
+            gave_up();
+            break;
+          }
+          const uint32_t l = stage0 + (uint32_t)(s * S::STAGE), tt = l + S::L_BYTES;
+          if constexpr (S::INNER) {
+            const bool cleared = kb == tile.k_blocks - 1 && tile.k_valid % S::MMA_STEP != 0;
+            const int boxes = (mine + 63) / 64, k = tile.k0 + kb * S::STEP;
+            const uint32_t bytes = (uint32_t)(S::L_BYTES + boxes * BOX_BYTES);
+            const uint32_t bar = cleared ? smem_u32(&bar_landed[s]) : leader_full + (uint32_t)(8 * s);
+            mbar_arrive_expect(bar, bytes);
+            tma_load_2d<S::CTAS>(l, &map_l, col, k, bar);
+            tma_load_2d<S::CTAS>(l + BOX_BYTES, &map_l, col + 64, k, bar);
+            for (int b = 0; b < boxes; ++b) tma_load_2d<S::CTAS>(tt + (uint32_t)(b * BOX_BYTES), &map_t, row + 64 * b, k, bar);
+          } else {
+            const uint32_t bar = leader_full + (uint32_t)(8 * s);
+            const int boxes = (mine + S::ROW_BOX - 1) / S::ROW_BOX, k = (tile.k0 + kb) * S::STEP;
+            mbar_arrive_expect(bar, (uint32_t)(S::L_BYTES + boxes * S::ROW_BOX * ROW_BYTES));
+            if constexpr (!S::MN) {
+              tma_load_3d<S::CTAS>(l, &map_l, k, col, tile.group, bar);
+            } else if constexpr (S::FP8) {
+              tma_load_3d<S::CTAS>(l, &map_l, col, k, tile.group, bar);
+            } else {
+              tma_load_3d<S::CTAS>(l, &map_l, col, k, tile.group, bar);
+              tma_load_3d<S::CTAS>(l + BOX_BYTES, &map_l, col + 64, k, tile.group, bar);
+            }
+            for (int b = 0; b < boxes; ++b)
+              tma_load_2d<S::CTAS>(tt + (uint32_t)(b * S::ROW_BOX * ROW_BYTES), &map_t, k, row + b * S::ROW_BOX, bar);
+          }
+          if (++s == S::STAGES) { s = 0; ++round; }
+        }
+      }
+      // the last arrivals on `empty` before the shared memory goes back
+      for (int i = 0; ok && i < S::STAGES; ++i) {
+        if (s == 0) {
+          if (round == 0) break;
+          s = S::STAGES;
+          --round;
+        }
+        --s;
+        ok = mbar_wait(smem_u32(&bar_empty[s]), round & 1u);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && (S::CTAS == 1 || rank == 0)) {
+      int s = 0, buffer = 0;
+      uint32_t round = 0, made = 0;  // accumulators begun
+      bool ok = true;
+      for (int t = walker; ok && t < tiles.total; t += walkers) {
+        const Tile tile = tiles.at(t, p, part, parts);
+        const uint32_t instruction = p.instruction | ((uint32_t)(tile.n >> 3) << 17);
+        uint32_t sums = 0;
+        for (int kb = 0; kb < tile.k_blocks; ++kb) {
+          const bool fresh = S::FP8 || kb == 0;
+          if (fresh) {
+            buffer = (int)(made % S::BUFFERS);
+            if (made >= S::BUFFERS) ok = mbar_wait(smem_u32(&bar_stored[buffer]), (made / S::BUFFERS - 1) & 1u);
+            sums = tmem + (uint32_t)(buffer * S::TILE);
+            ++made;
+          }
+          ok = ok && mbar_wait(smem_u32(&bar_full[s]), round & 1u);
+          if (!ok) {
+            gave_up();
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t l = stage0 + (uint32_t)(s * S::STAGE), tt = l + S::L_BYTES;
+          const int steps = S::INNER && kb == tile.k_blocks - 1 ? (tile.k_valid + S::MMA_STEP - 1) / S::MMA_STEP
+                                                                : S::STEP / S::MMA_STEP;
+#pragma unroll
+          for (int k = 0; k < S::STEP / S::MMA_STEP; ++k) {
+            if (S::INNER && k >= steps) break;
+            const uint64_t a = S::MN ? make_desc(l + (uint32_t)(k * S::MMA_STEP * ROW_BYTES), BOX_BYTES, 1024u)
+                                     : make_desc(l + (uint32_t)(k * 32), 16u, 1024u);
+            const uint64_t b = S::INNER ? make_desc(tt + (uint32_t)(k * S::MMA_STEP * ROW_BYTES), BOX_BYTES, 1024u)
+                                        : make_desc(tt + (uint32_t)(k * 32), 16u, 1024u);
+            issue_mma<S::CTAS, S::FP8>(sums, a, b, instruction, k > 0 || !fresh);
+          }
+          mma_commit<S::CTAS>(smem_u32(&bar_empty[s]));
+          if (S::FP8 || kb == tile.k_blocks - 1) mma_commit<S::CTAS>(smem_u32(&bar_sums[buffer]));
+          if (++s == S::STAGES) { s = 0; ++round; }
+        }
+      }
+    }
+  } else if (warp == 2) {
+    if constexpr (S::INNER) {
+      // The last stage of a group also holds rows behind the group's last: those that an MMA would read become zeros in both
+      // operands (only one would leave a product of zero and whatever the other rows hold).
+      uint32_t used = 0, turns = 0;  // stages copied so far; a bit per stage: parity of its turns here
+      bool ok = true;
+      const uint32_t leader_full = S::CTAS == 2 ? mapped(smem_u32(bar_full), 0) : smem_u32(bar_full);
+      for (int t = walker; ok && t < tiles.total; t += walkers) {
+        const Tile tile = tiles.at(t, p, part, parts);
+        used += (uint32_t)tile.k_blocks;
+        if (tile.k_blocks == 0 || tile.k_valid % S::MMA_STEP == 0) continue;
+        const int s = (int)((used - 1) % S::STAGES);
+        ok = mbar_wait(smem_u32(&bar_landed[s]), (turns >> s) & 1u);
+        ok = __all_sync(FULL, ok);
+        if (!ok) {
+          if (lane == 0) gave_up();
+          break;
+        }
+        turns ^= 1u << s;
+        const uint32_t base = stage0 + (uint32_t)(s * S::STAGE);
+        const int clear = (tile.k_valid + S::MMA_STEP - 1) / S::MMA_STEP * S::MMA_STEP - tile.k_valid;
+        constexpr int BOXES = S::STAGE / BOX_BYTES, PIECES = ROW_BYTES / 16;
+        for (int i = lane; i < clear * BOXES * PIECES; i += 32) {
+          const int piece = i % PIECES, box = i / PIECES % BOXES, row = tile.k_valid + i / (PIECES * BOXES);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + (uint32_t)(box * BOX_BYTES + row * ROW_BYTES + piece * 16)),
+                       "r"(0u) : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(leader_full + (uint32_t)(8 * s));
+      }
+    }
+  } else if (warp >= FIRST_STORE_WARP) {
+    const int store_warp = warp - FIRST_STORE_WARP, quarter = warp & 3;
+    const int c0 = store_warp / 4 * S::WARP_COLS;  // first accumulator column of this warp
+    const uint32_t lanes_at = (uint32_t)(quarter * 32) << 16;
+    uint32_t made = 0, shared_tiles = 0;
+    bool ok = true;
+    auto wait_sums = [&](int buffer) {
+      ok = mbar_wait(smem_u32(&bar_sums[buffer]), (made / S::BUFFERS) & 1u);
+      ok = __all_sync(FULL, ok);
+      if (!ok && lane == 0) gave_up();
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      return ok;
+    };
+    auto release_sums = [&](int buffer) {
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        const uint32_t bar = smem_u32(&bar_stored[buffer]);
+        mbar_arrive(S::CTAS == 2 ? mapped(bar, 0) : bar);
+      }
+      ++made;
+    };
+    for (int t = walker; ok && t < tiles.total; t += walkers) {
+      const Tile tile = tiles.at(t, p, part, parts);
+      const int col = tile.col0 + (S::CTAS == 2 ? rank * LANES : 0) + quarter * 32 + lane;
+      const bool stores = col < p.cols;
+      uint16_t *out = p.out + (S::INNER ? ((int64_t)tile.group * p.inner + tile.row0) * p.cols + col
+                                        : (int64_t)tile.row0 * p.cols + col);
+      if constexpr (!S::FP8) {
+        if (S::INNER && tile.k_blocks == 0) {  // a group without rows
+          if (stores)
+            for (int c = 0; c < tile.valid; ++c) out[(int64_t)c * p.cols] = 0;
+          continue;
+        }
+        const int buffer = (int)(made % S::BUFFERS);
+        if (!wait_sums(buffer)) break;
+        const bool split = S::SPLITS && parts > 1;
+        if (S::SPLITS && split && shared_tiles > 0) {  // the sums of the tile before have been read
+          ok = __all_sync(FULL, mbar_wait(smem_u32(&bar_added), (shared_tiles - 1) & 1u));
+          if (!ok) {
+            if (lane == 0) gave_up();
+            break;
+          }
+        }
+        for (int c = 0; c < tile.valid; c += 32) {
+          uint32_t v[32];
+          tmem_load(v, tmem + lanes_at + (uint32_t)(buffer * S::TILE + c));
+          tmem_wait_loads();
+          if (c + 32 >= tile.valid) release_sums(buffer);
+          if (split) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) partial[(c + i) * LANES + quarter * 32 + lane] = __uint_as_float(v[i]);
+          } else if (stores) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c + i < tile.valid) out[(int64_t)(c + i) * p.cols] = rounded(__uint_as_float(v[i]), p.half_out);
+          }
+        }
+      } else {
+        uint64_t sum[S::WARP_COLS / 2];
+#pragma unroll
+        for (int i = 0; i < S::WARP_COLS / 2; ++i) sum[i] = 0;
+        float *mine = scales + store_warp * 2 * S::WARP_COLS;
+        const float *b_scale = p.b_scales + (int64_t)tile.group * p.scale_group +
+                               (int64_t)((tile.col0 + (S::CTAS == 2 ? rank * LANES : 0)) / 128) * p.scale_j;
+        const bool any_col = tile.col0 + (S::CTAS == 2 ? rank * LANES : 0) < p.cols;
+        constexpr int PER_LANE = S::WARP_COLS / 32;
+        float next[PER_LANE];
+        auto fetch = [&](int kb) {
+          const int64_t block = tile.k0 + kb;
+          const float sb = any_col ? __ldg(b_scale + block * p.scale_k) : 0.0f;
+#pragma unroll
+          for (int i = 0; i < PER_LANE; ++i) {
+            const int c = c0 + i * 32 + lane;
+            next[i] = c < tile.valid ? sb * __ldg(p.a_scales + block * p.rows + tile.row0 + c) : 0.0f;
+          }
+        };
+        if (tile.k_blocks > 0) fetch(0);
+        for (int kb = 0; kb < tile.k_blocks; ++kb) {
+          float *here = mine + (kb & 1) * S::WARP_COLS;
+#pragma unroll
+          for (int i = 0; i < PER_LANE; ++i) here[i * 32 + lane] = next[i];
+          __syncwarp();
+          if (kb + 1 < tile.k_blocks) fetch(kb + 1);
+          const int buffer = (int)(made % S::BUFFERS);
+          if (!wait_sums(buffer)) break;
+#pragma unroll
+          for (int c = 0; c < S::WARP_COLS; c += 32) {
+            if (c0 + c < tile.valid) {
+              uint32_t v[32];
+              tmem_load(v, tmem + lanes_at + (uint32_t)(buffer * S::TILE + c0 + c));
+              tmem_wait_loads();
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(here + c + i);
+                sum[(c + i) / 2] = fma_two(pack(v[i], v[i + 1]), f.x, sum[(c + i) / 2]);
+                sum[(c + i) / 2 + 1] = fma_two(pack(v[i + 2], v[i + 3]), f.y, sum[(c + i) / 2 + 1]);
+              }
+            }
+          }
+          release_sums(buffer);
+        }
+        if (!ok) break;
+        if (S::SPLITS && parts > 1) {
+          if (shared_tiles > 0) {
+            ok = __all_sync(FULL, mbar_wait(smem_u32(&bar_added), (shared_tiles - 1) & 1u));
+            if (!ok) {
+              if (lane == 0) gave_up();
+              break;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < S::WARP_COLS; i += 2) {
+            uint32_t lo, hi;
+            unpack(sum[i / 2], lo, hi);
+            partial[(c0 + i) * LANES + quarter * 32 + lane] = __uint_as_float(lo);
+            partial[(c0 + i + 1) * LANES + quarter * 32 + lane] = __uint_as_float(hi);
+          }
+        } else if (stores) {
+#pragma unroll
+          for (int i = 0; i < S::WARP_COLS; i += 2) {
+            uint32_t lo, hi;
+            unpack(sum[i / 2], lo, hi);
+            if (c0 + i < tile.valid) out[(int64_t)(c0 + i) * p.cols] = rounded(__uint_as_float(lo), false);
+            if (c0 + i + 1 < tile.valid) out[(int64_t)(c0 + i + 1) * p.cols] = rounded(__uint_as_float(hi), false);
+          }
+        }
+      }
+      if constexpr (S::SPLITS) {
+        if (parts > 1) {
+          // Each warp's sums lie in its CTA's shared memory; the CTAs of the cluster add every `parts`-th column, in rank order.
+          __syncwarp();
+          if (lane < parts) mbar_arrive(mapped(smem_u32(&bar_parts), (uint32_t)lane));
+          ok = __all_sync(FULL, mbar_wait(smem_u32(&bar_parts), shared_tiles & 1u));
+          if (!ok) {
+            if (lane == 0) gave_up();
+            break;
+          }
+          const uint32_t at = smem_u32(partial) + (uint32_t)(quarter * 32 + lane) * 4u;
+          for (int c = part; c < tile.valid; c += parts) {
+            float total = 0.0f, v[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+              if (r < parts)
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[r]) : "r"(mapped(at + (uint32_t)(c * LANES * 4), (uint32_t)r)) : "memory");
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+              if (r < parts) total += v[r];
+            if (stores) out[(int64_t)c * p.cols] = rounded(total, p.half_out);
+          }
+          __syncwarp();
+          if (lane < parts) mbar_arrive(mapped(smem_u32(&bar_added), (uint32_t)lane));
+          ++shared_tiles;
+        }
+      }
+    }
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (failed) {
+    // A wait gave up with copies or MMAs possibly still in flight: give them a bounded time (1 ms) to land before the shared
+    // memory and the TMEM columns go back to the SM.
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  }
+  if (S::CTAS == 2 || parts > 1)  // no CTA leaves while another may use its shared memory, barriers or TMEM
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 1) {
+    if constexpr (S::CTAS == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM_COLS) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM_COLS) : "memory");
+  }
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled_fn() {
+  static EncodeTiledFn fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                       q == cudaDriverEntryPointSuccess;
+    return found ? reinterpret_cast<EncodeTiledFn>(p) : nullptr;
+  }();
+  return fn;
+}
+
+// `stack` matrices of `outer` rows of `inner` contiguous elements (rank 2 without a stack), boxes of 128 swizzled bytes x box_rows.
+bool make_map(CUtensorMap *map, const void *base, int type, int64_t inner, int64_t outer, int64_t stack, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  const cuuint64_t size = type == kBF16 || type == kF16 ? 2 : 1;
+  cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)stack};
+  cuuint64_t strides[2] = {(cuuint64_t)inner * size, (cuuint64_t)(inner * outer) * size};
+  cuuint32_t box[3] = {(cuuint32_t)(ROW_BYTES / size), box_rows, 1};
+  cuuint32_t elem[3] = {1, 1, 1};
+  const CUtensorMapDataType data = type == kBF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                   : type == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  return fn(map, data, stack > 0 ? 3 : 2, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Opts a kernel into its shared memory, once per device; racing threads repeat an idempotent call.
+template <class S>
+cudaError_t configure() {
+  static std::atomic<bool> configured[64];
+  int device = 0;
+  cudaGetDevice(&device);
+  if (device >= 0 && device < 64 && configured[device].load(std::memory_order_acquire)) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(grouped_tcgen05_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+  if (e == cudaSuccess && device >= 0 && device < 64) configured[device].store(true, std::memory_order_release);
+  return e;
+}
+
+template <class S>
+cudaError_t launch(const CUtensorMap &map_l, const CUtensorMap &map_t, const Product &p, int64_t most_tiles, int parts, int sm_count,
+                   cudaStream_t s) {
+  if (most_tiles == 0) return cudaSuccess;
+  if (most_tiles > 2147483647LL - 4096) return cudaErrorInvalidConfiguration;  // tile numbers are 32-bit
+  cudaError_t e = configure<S>();
+  if (e != cudaSuccess) return e;
+  const int cluster = S::CTAS == 2 ? 2 : parts;
+  const int64_t walkers = most_tiles < sm_count / cluster ? most_tiles : sm_count / cluster;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = (unsigned)cluster;
+  attributes[1].val.clusterDim.y = 1;
+  attributes[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(walkers * cluster));
+  cfg.blockDim = dim3(S::THREADS);
+  cfg.dynamicSmemBytes = S::SMEM;
+  cfg.stream = s;
+  cfg.attrs = attributes;
+  cfg.numAttrs = 2;
+  e = cudaLaunchKernelEx(&cfg, grouped_tcgen05_kernel<S>, map_l, map_t, p, parts);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// kind::f16 and kind::f8f6f4: f32 sums (bits 4-5), types of A and B (bits 7-9, 10-12), MN-major A and B (bits 15, 16),
+// N >> 3 (bits 17-22, per tile), M >> 4 (bits 24-28).
+uint32_t instruction_descriptor(int a_type, int b_type, bool a_mn, bool b_mn, int m) {
+  auto code = [](int type) { return type == kBF16 || type == kE5M2 ? 1u : 0u; };
+  return (1u << 4) | (code(a_type) << 7) | (code(b_type) << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
+         ((uint32_t)(m >> 4) << 24);
+}
+
+template <int CTAS, int TILE, bool FP8, bool MN>
+cudaError_t launch_rows(const GroupedArgs &a, Product p, int parts, const DeviceInfo &dev, cudaStream_t s) {
+  using S = Config<CTAS, TILE, FP8, MN, false>;
+  CUtensorMap map_l, map_t;
+  const int b_type = FP8 ? a.b_type : a.type;
+  const bool made = (MN ? make_map(&map_l, a.B, b_type, a.n, a.inner, a.groups, S::STEP)
+                        : make_map(&map_l, a.B, b_type, a.inner, a.n, a.groups, LANES)) &&
+                    make_map(&map_t, a.A, a.type, a.inner, a.rows, 0, S::ROW_BOX);
+  if (!made) return cudaErrorInvalidValue;
+  p.instruction = instruction_descriptor(b_type, a.type, MN, false, LANES * CTAS);
+  const int64_t most = (ceil_div(a.rows, TILE) + (a.groups < a.rows ? a.groups : a.rows)) * ceil_div(a.n, LANES * CTAS);
+  return launch<S>(map_l, map_t, p, most, parts, dev.sm_count, s);
+}
+
+// Narrow tiles where groups have few rows.
+constexpr int64_t NARROW_ROWS = 64;
+
+}  // namespace
+
+bool grouped_rows_tcgen05_supported(const GroupedArgs &a) {
+  const int64_t size = a.a_scales ? 1 : 2, pitch = a.transpose_b ? a.inner : a.n;
+  return a.inner > 0 && a.rows > 0 && a.inner * size % 16 == 0 && pitch * size % 16 == 0 && aligned16(a.A) && aligned16(a.B);
+}
+
+cudaError_t launch_grouped_rows_tcgen05(const GroupedArgs &a, int *status_flag, const DeviceInfo &dev, cudaStream_t s,
+                                        int64_t *launches) {
+  ++*launches;
+  Product p = {};
+  p.rows = (int)a.rows;
+  p.inner = (int)a.inner;
+  p.cols = (int)a.n;
+  p.groups = (int)a.groups;
+  p.offsets = a.offsets;
+  p.out = static_cast<uint16_t *>(a.C);
+  p.half_out = !a.a_scales && a.type == kF16;
+  p.a_scales = a.a_scales;
+  p.b_scales = a.b_scales;
+  const int64_t kb = ceil_div(a.inner, kScaleBlock), nb = ceil_div(a.n, kScaleBlock);
+  p.scale_k = (int)(a.transpose_b ? 1 : nb);
+  p.scale_j = (int)(a.transpose_b ? kb : 1);
+  p.scale_group = (int)(kb * nb);
+  p.status = status_flag;
+  const int64_t active = a.groups < a.rows ? a.groups : a.rows;
+  if (a.rows <= NARROW_ROWS * active) {
+    const int64_t tiles = active * ceil_div(a.n, LANES), steps = ceil_div(a.inner, a.a_scales ? 128 : 64);
+    int parts = 1;
+    while (parts < 8 && tiles * parts * 2 <= dev.sm_count && steps >= parts * 4) parts *= 2;
+    if (a.a_scales)
+      return a.transpose_b ? launch_rows<1, 64, true, false>(a, p, parts, dev, s) : launch_rows<1, 64, true, true>(a, p, parts, dev, s);
+    return a.transpose_b ? launch_rows<1, 64, false, false>(a, p, parts, dev, s) : launch_rows<1, 64, false, true>(a, p, parts, dev, s);
+  }
+  if (a.a_scales)
+    return a.transpose_b ? launch_rows<2, 256, true, false>(a, p, 1, dev, s) : launch_rows<2, 256, true, true>(a, p, 1, dev, s);
+  return a.transpose_b ? launch_rows<2, 256, false, false>(a, p, 1, dev, s) : launch_rows<2, 256, false, true>(a, p, 1, dev, s);
+}
+
+bool grouped_inner_tcgen05_supported(const GroupedInnerArgs &a) {
+  return a.rows > 0 && a.i_size % 8 == 0 && a.j_size % 8 == 0 && aligned16(a.left) && aligned16(a.right);
+}
+
+cudaError_t launch_grouped_inner_tcgen05(const GroupedInnerArgs &a, int *status_flag, const DeviceInfo &dev, cudaStream_t s,
+                                         int64_t *launches) {
+  ++*launches;
+  using S = Config<2, 256, false, true, true>;
+  CUtensorMap map_l, map_t;
+  if (!make_map(&map_l, a.right, a.type, a.j_size, a.rows, 0, S::STEP) || !make_map(&map_t, a.left, a.type, a.i_size, a.rows, 0, S::ROW_BOX))
+    return cudaErrorInvalidValue;
+  Product p = {};
+  p.rows = (int)a.rows;
+  p.inner = (int)a.i_size;
+  p.cols = (int)a.j_size;
+  p.groups = (int)a.groups;
+  p.offsets = a.offsets;
+  p.out = static_cast<uint16_t *>(a.out);
+  p.half_out = a.type == kF16;
+  p.status = status_flag;
+  p.instruction = instruction_descriptor(a.type, a.type, true, true, LANES * 2);
+  const int64_t tiles = a.groups * ceil_div(a.i_size, S::TILE) * ceil_div(a.j_size, LANES * 2);
+  return launch<S>(map_l, map_t, p, tiles, 1, dev.sm_count, s);
+}
+
+}  // namespace swb

@@ -45,6 +45,21 @@ int check_grouped(swb_context *ctx, const char *op, int64_t rows, int64_t inner,
   return SWB_OK;
 }
 
+cudaError_t rows_product(swb_context *ctx, const swb::GroupedArgs &a, swb_stream stream) {
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int64_t *launches = swb::context_launches(ctx);
+  return swb::grouped_rows_tcgen05_supported(a)
+             ? swb::launch_grouped_rows_tcgen05(a, swb::context_status_flag(ctx), swb::context_device_info(ctx), s, launches)
+             : swb::launch_grouped_rows_general(a, s, launches);
+}
+cudaError_t inner_product(swb_context *ctx, const swb::GroupedInnerArgs &a, swb_stream stream) {
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int64_t *launches = swb::context_launches(ctx);
+  return swb::grouped_inner_tcgen05_supported(a)
+             ? swb::launch_grouped_inner_tcgen05(a, swb::context_status_flag(ctx), swb::context_device_info(ctx), s, launches)
+             : swb::launch_grouped_inner_general(a, s, launches);
+}
+
 bool is_fp8(int32_t type) { return type == SWB_E4M3 || type == SWB_E5M2; }
 
 int fp8_product(swb_context *ctx, const char *op, int32_t a_type, int32_t b_type, int64_t rows, int64_t inner, int64_t n,
@@ -59,7 +74,7 @@ int fp8_product(swb_context *ctx, const char *op, int32_t a_type, int32_t b_type
   a.b_type = b_type;
   a.a_scales = a_scales;
   a.b_scales = b_scales;
-  return cuda_status(ctx, swb::launch_grouped_rows_general(a, static_cast<cudaStream_t>(stream), swb::context_launches(ctx)), op);
+  return cuda_status(ctx, rows_product(ctx, a, stream), op);
 }
 
 int quantize(swb_context *ctx, const char *op, bool by_rows, int32_t type, int32_t fp8_type, int64_t groups, int64_t rows,
@@ -101,8 +116,7 @@ int swb_grouped_mm(swb_context *ctx, int32_t dtype, int64_t rows, int64_t inner,
   if (!offsets || (rows > 0 && inner > 0 && !A) || (inner > 0 && !B) || (rows > 0 && !C))
     return fail(ctx, SWB_ERR_INVALID_ARGUMENT, "grouped_mm: NULL operand pointer");
   const swb::GroupedArgs a{rows, inner, n, groups, offsets, A, B, transpose_b != 0, C, dtype};
-  return cuda_status(ctx, swb::launch_grouped_rows_general(a, static_cast<cudaStream_t>(stream), swb::context_launches(ctx)),
-                     "grouped_mm");
+  return cuda_status(ctx, rows_product(ctx, a, stream), "grouped_mm");
 }
 
 int swb_grouped_mm_grad(swb_context *ctx, int32_t dtype, int64_t rows, int64_t inner, int64_t n, int64_t groups,
@@ -117,17 +131,15 @@ int swb_grouped_mm_grad(swb_context *ctx, int32_t dtype, int64_t rows, int64_t i
     return fail(ctx, SWB_ERR_INVALID_ARGUMENT, "grouped_mm_grad: operands must be bf16 or f16, but got type %d", dtype);
   if (!offsets || (rows > 0 && (!dC || (dB && !A))) || (rows > 0 && dA && !B))
     return fail(ctx, SWB_ERR_INVALID_ARGUMENT, "grouped_mm_grad: NULL operand pointer");
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int64_t *launches = swb::context_launches(ctx);
   if (dA) {  // dA = dC B^T: the same product with the weights read the other way round
     const swb::GroupedArgs a{rows, n, inner, groups, offsets, dC, B, transpose_b == 0, dA, dtype};
-    st = cuda_status(ctx, swb::launch_grouped_rows_general(a, s, launches), "grouped_mm_grad");
+    st = cuda_status(ctx, rows_product(ctx, a, stream), "grouped_mm_grad");
     if (st != SWB_OK) return st;
   }
   if (dB) {
     const swb::GroupedInnerArgs a = transpose_b ? swb::GroupedInnerArgs{rows, n, inner, groups, offsets, dC, A, dB, dtype}
                                                 : swb::GroupedInnerArgs{rows, inner, n, groups, offsets, A, dC, dB, dtype};
-    st = cuda_status(ctx, swb::launch_grouped_inner_general(a, s, launches), "grouped_mm_grad");
+    st = cuda_status(ctx, inner_product(ctx, a, stream), "grouped_mm_grad");
   }
   return st;
 }

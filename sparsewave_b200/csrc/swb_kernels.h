@@ -181,6 +181,13 @@ cudaError_t launch_bsr_spmm_tcgen05(const BsrSpmmArgs &a, int *status_flag, cons
 // --- products grouped by expert, 8-bit operands
 cudaError_t launch_grouped_rows_general(const GroupedArgs &a, cudaStream_t s, int64_t *launches);
 cudaError_t launch_grouped_inner_general(const GroupedInnerArgs &a, cudaStream_t s, int64_t *launches);
+// The same on the tcgen05 tensor cores: operands and their rows on 16-byte boundaries, an inner axis.  `status_flag` as for BSR.
+bool grouped_rows_tcgen05_supported(const GroupedArgs &a);
+cudaError_t launch_grouped_rows_tcgen05(const GroupedArgs &a, int *status_flag, const DeviceInfo &dev, cudaStream_t s,
+                                        int64_t *launches);
+bool grouped_inner_tcgen05_supported(const GroupedInnerArgs &a);
+cudaError_t launch_grouped_inner_tcgen05(const GroupedInnerArgs &a, int *status_flag, const DeviceInfo &dev, cudaStream_t s,
+                                         int64_t *launches);
 cudaError_t launch_quantize_rows(const QuantizeArgs &a, cudaStream_t s, int64_t *launches);
 cudaError_t launch_quantize_blocks(const QuantizeArgs &a, cudaStream_t s, int64_t *launches);
 
