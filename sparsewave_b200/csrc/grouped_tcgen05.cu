@@ -84,14 +84,24 @@ __device__ __forceinline__ uint64_t make_desc(uint32_t addr, uint32_t lbo_bytes,
          ((uint64_t)((sbo_bytes >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// Copies, MMAs and accumulators are ordered by their own rules, so that a wait needs to see plain stores of its own CTA at most;
+// CLUSTER: stores of other CTAs too.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
   for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
     uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    if constexpr (CLUSTER)
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    else
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     if (done) return true;
   }
   return false;
@@ -99,12 +109,16 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-// `bar` may be another CTA's of the cluster (mapped).
+// `bar` may be another CTA's of the cluster (mapped).  RELEASE: the warp's plain stores before it are visible to who waits.
+template <bool RELEASE = false>
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  if constexpr (RELEASE)
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ uint32_t mapped(uint32_t addr, uint32_t rank) {  // the same place in CTA `rank` of the cluster
   uint32_t out;
@@ -466,7 +480,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(leader_full + (uint32_t)(8 * s));
+        if (lane == 0) mbar_arrive<true>(leader_full + (uint32_t)(8 * s));
       }
     }
   } else if (warp >= FIRST_STORE_WARP) {
@@ -507,7 +521,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
         if (!wait_sums(buffer)) break;
         const bool split = S::SPLITS && parts > 1;
         if (S::SPLITS && split && shared_tiles > 0) {  // the sums of the tile before have been read
-          ok = __all_sync(FULL, mbar_wait(smem_u32(&bar_added), (shared_tiles - 1) & 1u));
+          ok = __all_sync(FULL, mbar_wait<true>(smem_u32(&bar_added), (shared_tiles - 1) & 1u));
           if (!ok) {
             if (lane == 0) gave_up();
             break;
@@ -574,7 +588,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
         if (!ok) break;
         if (S::SPLITS && parts > 1) {
           if (shared_tiles > 0) {
-            ok = __all_sync(FULL, mbar_wait(smem_u32(&bar_added), (shared_tiles - 1) & 1u));
+            ok = __all_sync(FULL, mbar_wait<true>(smem_u32(&bar_added), (shared_tiles - 1) & 1u));
             if (!ok) {
               if (lane == 0) gave_up();
               break;
@@ -601,8 +615,8 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
         if (parts > 1) {
           // Each warp's sums lie in its CTA's shared memory; the CTAs of the cluster add every `parts`-th column, in rank order.
           __syncwarp();
-          if (lane < parts) mbar_arrive(mapped(smem_u32(&bar_parts), (uint32_t)lane));
-          ok = __all_sync(FULL, mbar_wait(smem_u32(&bar_parts), shared_tiles & 1u));
+          if (lane < parts) mbar_arrive<true>(mapped(smem_u32(&bar_parts), (uint32_t)lane));
+          ok = __all_sync(FULL, mbar_wait<true>(smem_u32(&bar_parts), shared_tiles & 1u));
           if (!ok) {
             if (lane == 0) gave_up();
             break;
@@ -620,7 +634,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
             if (stores) out[(int64_t)c * p.cols] = rounded(total, p.half_out);
           }
           __syncwarp();
-          if (lane < parts) mbar_arrive(mapped(smem_u32(&bar_added), (uint32_t)lane));
+          if (lane < parts) mbar_arrive<true>(mapped(smem_u32(&bar_added), (uint32_t)lane));
           ++shared_tiles;
         }
       }
