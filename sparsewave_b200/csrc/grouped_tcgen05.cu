@@ -15,7 +15,7 @@
 // Which tile lies where is worked out on the device from the offsets: every CTA builds the table of the groups' tiles in shared
 // memory, and the CTAs (pairs, clusters) walk the tiles in turn.
 //
-// Roles: lane 0 of warp 0 copies, lane 0 of warp 1 issues the MMAs, warp 2 clears the rows behind a group's last (inner form),
+// Roles: warp 0 copies, warp 1 issues the MMAs, warp 2 clears the rows behind a group's last (inner form),
 // four warps (wide 8-bit: eight) from warp 4 on read the accumulators, round and store.
 //
 // 8-bit operands: the 128 products of a scale block are one chain of the tensor core in an accumulator of its own; the storing
@@ -82,6 +82,12 @@ __device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast
 __device__ __forceinline__ uint64_t make_desc(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {  // 128-byte swizzle
   return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo_bytes >> 4) & 0x3FFFu) << 16) |
          ((uint64_t)((sbo_bytes >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ bool elected() {  // one lane of a converged warp
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
 // Copies, MMAs and accumulators are ordered by their own rules, so that a wait needs to see plain stores of its own CTA at most;
@@ -212,6 +218,19 @@ struct Tile {
   int k0, k_blocks, k_valid;  // first stage of the inner axis, stages, elements of the last that exist
 };
 
+__device__ __forceinline__ Tile uniform(const Tile &t) {  // the same in all lanes, known to be
+  Tile u;
+  u.group = __shfl_sync(FULL, t.group, 0);
+  u.row0 = __shfl_sync(FULL, t.row0, 0);
+  u.valid = __shfl_sync(FULL, t.valid, 0);
+  u.n = __shfl_sync(FULL, t.n, 0);
+  u.col0 = __shfl_sync(FULL, t.col0, 0);
+  u.k0 = __shfl_sync(FULL, t.k0, 0);
+  u.k_blocks = __shfl_sync(FULL, t.k_blocks, 0);
+  u.k_valid = __shfl_sync(FULL, t.k_valid, 0);
+  return u;
+}
+
 template <class S>
 struct Tiles {
   const int2 *spans;
@@ -270,7 +289,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(FULL, tid >> 5, 0), lane = tid & 31;
   const uint32_t stage0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t *behind = smem_raw + (stage0 - smem_u32(smem_raw)) + S::STAGES * S::STAGE;
   float *partial = reinterpret_cast<float *>(behind);                         // [TILE][LANES]
@@ -347,76 +366,81 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   }
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = tmem_slot;
-  tiles.total = S::INNER ? p.groups * tiles.col_tiles * tiles.inner_tiles : first[p.groups];
+  const uint32_t tmem = __shfl_sync(FULL, tmem_slot, 0);
+  tiles.total = S::INNER ? p.groups * tiles.col_tiles * tiles.inner_tiles : __shfl_sync(FULL, first[p.groups], 0);
 
   auto gave_up = [&] {
     failed = 1;
     atomicExch(p.status, 1);
   };
 
+  // The warps that copy and that issue MMAs walk their loops as whole warps and elect a lane for the instructions alone: what these
+  // take then lies in uniform registers (as one lane's own code, four MMAs took their thread 690 clocks whatever their size).
   if (warp == 0) {
-    if (lane == 0) {
-      int s = 0;
-      uint32_t round = 0;
-      bool ok = true;
-      const uint32_t leader_full = S::CTAS == 2 ? mapped(smem_u32(bar_full), 0) : smem_u32(bar_full);
-      for (int t = walker; ok && t < tiles.total; t += walkers) {
-        const Tile tile = tiles.at(t, p, part, parts);
-        const int mine = tile.n / S::CTAS, row = tile.row0 + (S::CTAS == 2 ? rank * mine : 0);
-        const int col = tile.col0 + (S::CTAS == 2 ? rank * LANES : 0);
-        for (int kb = 0; kb < tile.k_blocks; ++kb) {
-          if (round > 0) ok = mbar_wait(smem_u32(&bar_empty[s]), (round - 1) & 1u);
-          if (!ok) {
-            gave_up();
-            break;
-          }
-          const uint32_t l = stage0 + (uint32_t)(s * S::STAGE), tt = l + S::L_BYTES;
-          if constexpr (S::INNER) {
-            const bool cleared = kb == tile.k_blocks - 1 && tile.k_valid % S::MMA_STEP != 0;
-            const int boxes = (mine + 63) / 64, k = tile.k0 + kb * S::STEP;
-            const uint32_t bytes = (uint32_t)(S::L_BYTES + boxes * BOX_BYTES);
-            const uint32_t bar = cleared ? smem_u32(&bar_landed[s]) : leader_full + (uint32_t)(8 * s);
+    int s = 0;
+    uint32_t round = 0;
+    bool ok = true;
+    const bool issues = elected();
+    const uint32_t leader_full = S::CTAS == 2 ? mapped(smem_u32(bar_full), 0) : smem_u32(bar_full);
+    for (int t = walker; ok && t < tiles.total; t += walkers) {
+      const Tile tile = uniform(tiles.at(t, p, part, parts));
+      const int mine = tile.n / S::CTAS, row = tile.row0 + (S::CTAS == 2 ? rank * mine : 0);
+      const int col = tile.col0 + (S::CTAS == 2 ? rank * LANES : 0);
+      const int boxes = (mine + S::ROW_BOX - 1) / S::ROW_BOX;
+      const uint32_t bytes = (uint32_t)(S::L_BYTES + boxes * S::ROW_BOX * ROW_BYTES);
+      for (int kb = 0; kb < tile.k_blocks; ++kb) {
+        if (round > 0) ok = __all_sync(FULL, mbar_wait(smem_u32(&bar_empty[s]), (round - 1) & 1u));
+        if (!ok) {
+          if (issues) gave_up();
+          break;
+        }
+        const uint32_t l = stage0 + (uint32_t)(s * S::STAGE), tt = l + S::L_BYTES;
+        uint32_t bar = leader_full + (uint32_t)(8 * s);
+        if constexpr (S::INNER) {
+          if (kb == tile.k_blocks - 1 && tile.k_valid % S::MMA_STEP != 0) bar = smem_u32(&bar_landed[s]);
+          const int k = tile.k0 + kb * S::STEP;
+          if (issues) {
             mbar_arrive_expect(bar, bytes);
             tma_load_2d<S::CTAS>(l, &map_l, col, k, bar);
             tma_load_2d<S::CTAS>(l + BOX_BYTES, &map_l, col + 64, k, bar);
             for (int b = 0; b < boxes; ++b) tma_load_2d<S::CTAS>(tt + (uint32_t)(b * BOX_BYTES), &map_t, row + 64 * b, k, bar);
-          } else {
-            const uint32_t bar = leader_full + (uint32_t)(8 * s);
-            const int boxes = (mine + S::ROW_BOX - 1) / S::ROW_BOX, k = (tile.k0 + kb) * S::STEP;
-            mbar_arrive_expect(bar, (uint32_t)(S::L_BYTES + boxes * S::ROW_BOX * ROW_BYTES));
+          }
+        } else {
+          const int k = (tile.k0 + kb) * S::STEP;
+          if (issues) {
+            mbar_arrive_expect(bar, bytes);
             if constexpr (!S::MN) {
               tma_load_3d<S::CTAS>(l, &map_l, k, col, tile.group, bar);
-            } else if constexpr (S::FP8) {
-              tma_load_3d<S::CTAS>(l, &map_l, col, k, tile.group, bar);
             } else {
               tma_load_3d<S::CTAS>(l, &map_l, col, k, tile.group, bar);
-              tma_load_3d<S::CTAS>(l + BOX_BYTES, &map_l, col + 64, k, tile.group, bar);
+              if constexpr (!S::FP8) tma_load_3d<S::CTAS>(l + BOX_BYTES, &map_l, col + 64, k, tile.group, bar);
             }
             for (int b = 0; b < boxes; ++b)
               tma_load_2d<S::CTAS>(tt + (uint32_t)(b * S::ROW_BOX * ROW_BYTES), &map_t, k, row + b * S::ROW_BOX, bar);
           }
-          if (++s == S::STAGES) { s = 0; ++round; }
         }
-      }
-      // the last arrivals on `empty` before the shared memory goes back
-      for (int i = 0; ok && i < S::STAGES; ++i) {
-        if (s == 0) {
-          if (round == 0) break;
-          s = S::STAGES;
-          --round;
-        }
-        --s;
-        ok = mbar_wait(smem_u32(&bar_empty[s]), round & 1u);
+        __syncwarp();
+        if (++s == S::STAGES) { s = 0; ++round; }
       }
     }
+    // the last arrivals on `empty` before the shared memory goes back
+    for (int i = 0; ok && i < S::STAGES; ++i) {
+      if (s == 0) {
+        if (round == 0) break;
+        s = S::STAGES;
+        --round;
+      }
+      --s;
+      ok = mbar_wait(smem_u32(&bar_empty[s]), round & 1u);
+    }
   } else if (warp == 1) {
-    if (lane == 0 && (S::CTAS == 1 || rank == 0)) {
+    if (S::CTAS == 1 || rank == 0) {
       int s = 0, buffer = 0;
       uint32_t round = 0, made = 0;  // accumulators begun
       bool ok = true;
+      const bool issues = elected();
       for (int t = walker; ok && t < tiles.total; t += walkers) {
-        const Tile tile = tiles.at(t, p, part, parts);
+        const Tile tile = uniform(tiles.at(t, p, part, parts));
         const uint32_t instruction = p.instruction | ((uint32_t)(tile.n >> 3) << 17);
         uint32_t sums = 0;
         for (int kb = 0; kb < tile.k_blocks; ++kb) {
@@ -427,26 +451,27 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
             sums = tmem + (uint32_t)(buffer * S::TILE);
             ++made;
           }
-          ok = ok && mbar_wait(smem_u32(&bar_full[s]), round & 1u);
+          ok = __all_sync(FULL, ok && mbar_wait(smem_u32(&bar_full[s]), round & 1u));
           if (!ok) {
-            gave_up();
+            if (issues) gave_up();
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t l = stage0 + (uint32_t)(s * S::STAGE), tt = l + S::L_BYTES;
-          const int steps = S::INNER && kb == tile.k_blocks - 1 ? (tile.k_valid + S::MMA_STEP - 1) / S::MMA_STEP
-                                                                : S::STEP / S::MMA_STEP;
+          const bool last = kb == tile.k_blocks - 1;
+          const int steps = S::INNER && last ? (tile.k_valid + S::MMA_STEP - 1) / S::MMA_STEP : S::STEP / S::MMA_STEP;
+          const uint64_t a = S::MN ? make_desc(l, BOX_BYTES, 1024u) : make_desc(l, 16u, 1024u);
+          const uint64_t b = S::INNER ? make_desc(tt, BOX_BYTES, 1024u) : make_desc(tt, 16u, 1024u);
+          constexpr uint64_t A_STEP = S::MN ? S::MMA_STEP * ROW_BYTES / 16 : 2, B_STEP = S::INNER ? S::MMA_STEP * ROW_BYTES / 16 : 2;
+          if (issues) {
 #pragma unroll
-          for (int k = 0; k < S::STEP / S::MMA_STEP; ++k) {
-            if (S::INNER && k >= steps) break;
-            const uint64_t a = S::MN ? make_desc(l + (uint32_t)(k * S::MMA_STEP * ROW_BYTES), BOX_BYTES, 1024u)
-                                     : make_desc(l + (uint32_t)(k * 32), 16u, 1024u);
-            const uint64_t b = S::INNER ? make_desc(tt + (uint32_t)(k * S::MMA_STEP * ROW_BYTES), BOX_BYTES, 1024u)
-                                        : make_desc(tt + (uint32_t)(k * 32), 16u, 1024u);
-            issue_mma<S::CTAS, S::FP8>(sums, a, b, instruction, k > 0 || !fresh);
+            for (int k = 0; k < S::STEP / S::MMA_STEP; ++k)
+              if (!S::INNER || k < steps)
+                issue_mma<S::CTAS, S::FP8>(sums, a + (uint64_t)k * A_STEP, b + (uint64_t)k * B_STEP, instruction, k > 0 || !fresh);
+            mma_commit<S::CTAS>(smem_u32(&bar_empty[s]));
+            if (S::FP8 || last) mma_commit<S::CTAS>(smem_u32(&bar_sums[buffer]));
           }
-          mma_commit<S::CTAS>(smem_u32(&bar_empty[s]));
-          if (S::FP8 || kb == tile.k_blocks - 1) mma_commit<S::CTAS>(smem_u32(&bar_sums[buffer]));
+          __syncwarp();
           if (++s == S::STAGES) { s = 0; ++round; }
         }
       }
