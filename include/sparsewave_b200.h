@@ -332,9 +332,9 @@ SWB_API int swb_grouped_mm_grad(swb_context *ctx, int32_t dtype, int64_t rows,
                                 int32_t transpose_b, void *dA, void *dB,
                                 swb_stream stream);
 
-/* 8-bit values with a scale for each block of 128: q = x / scale rounded to
- * fp8_dtype (SWB_E4M3 or SWB_E5M2), scale = max |x| of the block / the largest
- * value of fp8_dtype, at least 2^-126.  `dtype` is that of X: SWB_BF16,
+/* 8-bit values with a scale for each block of 128: q = x * (1 / scale) rounded
+ * to fp8_dtype (SWB_E4M3 or SWB_E5M2), scale = max |x| of the block / the
+ * largest value of fp8_dtype, at least 2^-126.  `dtype` is that of X: SWB_BF16,
  * SWB_F16 or SWB_F32.  A block with a NaN or an infinity gets that as its
  * scale, and every product with it is NaN.
  *

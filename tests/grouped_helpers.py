@@ -79,7 +79,7 @@ def quantize_rows(X, dtype=torch.float8_e4m3fn):
     x = torch.nn.functional.pad(X.float(), (0, -X.shape[1] % BLOCK))
     amax = x.abs().view(X.shape[0], -1, BLOCK).amax(2)
     scales = scale_of(amax, dtype).t().contiguous()
-    return (X.float() / spread_rows(scales, X.shape[1])).to(dtype), scales
+    return (X.float() * spread_rows(1.0 / scales, X.shape[1])).to(dtype), scales
 
 
 def quantize_blocks(X, dtype=torch.float8_e4m3fn):
@@ -88,7 +88,7 @@ def quantize_blocks(X, dtype=torch.float8_e4m3fn):
     x = torch.nn.functional.pad(stack.float(), (0, -c % BLOCK, 0, -r % BLOCK))
     amax = x.abs().view(g, x.shape[1] // BLOCK, BLOCK, -1, BLOCK).amax((2, 4))
     scales = scale_of(amax, dtype)
-    q = (stack.float() / spread_blocks(scales, r, c)).to(dtype)
+    q = (stack.float() * spread_blocks(1.0 / scales, r, c)).to(dtype)
     return (q, scales) if X.dim() == 3 else (q[0], scales[0])
 
 
