@@ -376,139 +376,145 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
 
   // The warps that copy and that issue MMAs walk their loops as whole warps and elect a lane for the instructions alone: what these
   // take then lies in uniform registers (as one lane's own code, four MMAs took their thread 690 clocks whatever their size).
-  if (warp == 0) {
-    int s = 0;
-    uint32_t round = 0;
-    bool ok = true;
-    const bool issues = elected();
-    const uint32_t leader_full = S::CTAS == 2 ? mapped(smem_u32(bar_full), 0) : smem_u32(bar_full);
-    for (int t = walker; ok && t < tiles.total; t += walkers) {
-      const Tile tile = uniform(tiles.at(t, p, part, parts));
-      const int mine = tile.n / S::CTAS, row = tile.row0 + (S::CTAS == 2 ? rank * mine : 0);
-      const int col = tile.col0 + (S::CTAS == 2 ? rank * LANES : 0);
-      const int boxes = (mine + S::ROW_BOX - 1) / S::ROW_BOX;
-      const uint32_t bytes = (uint32_t)(S::L_BYTES + boxes * S::ROW_BOX * ROW_BYTES);
-      for (int kb = 0; kb < tile.k_blocks; ++kb) {
-        if (round > 0) ok = __all_sync(FULL, mbar_wait(smem_u32(&bar_empty[s]), (round - 1) & 1u));
-        if (!ok) {
-          if (issues) gave_up();
-          break;
-        }
-        const uint32_t l = stage0 + (uint32_t)(s * S::STAGE), tt = l + S::L_BYTES;
-        uint32_t bar = leader_full + (uint32_t)(8 * s);
-        if constexpr (S::INNER) {
-          if (kb == tile.k_blocks - 1 && tile.k_valid % S::MMA_STEP != 0) bar = smem_u32(&bar_landed[s]);
-          const int k = tile.k0 + kb * S::STEP;
-          if (issues) {
-            mbar_arrive_expect(bar, bytes);
-            tma_load_2d<S::CTAS>(l, &map_l, col, k, bar);
-            tma_load_2d<S::CTAS>(l + BOX_BYTES, &map_l, col + 64, k, bar);
-            for (int b = 0; b < boxes; ++b) tma_load_2d<S::CTAS>(tt + (uint32_t)(b * BOX_BYTES), &map_t, row + 64 * b, k, bar);
-          }
-        } else {
-          const int k = (tile.k0 + kb) * S::STEP;
-          if (issues) {
-            mbar_arrive_expect(bar, bytes);
-            if constexpr (!S::MN) {
-              tma_load_3d<S::CTAS>(l, &map_l, k, col, tile.group, bar);
-            } else {
-              tma_load_3d<S::CTAS>(l, &map_l, col, k, tile.group, bar);
-              if constexpr (!S::FP8) tma_load_3d<S::CTAS>(l + BOX_BYTES, &map_l, col + 64, k, tile.group, bar);
-            }
-            for (int b = 0; b < boxes; ++b)
-              tma_load_2d<S::CTAS>(tt + (uint32_t)(b * S::ROW_BOX * ROW_BYTES), &map_t, k, row + b * S::ROW_BOX, bar);
-          }
-        }
-        __syncwarp();
-        if (++s == S::STAGES) { s = 0; ++round; }
-      }
-    }
-    // the last arrivals on `empty` before the shared memory goes back
-    for (int i = 0; ok && i < S::STAGES; ++i) {
-      if (s == 0) {
-        if (round == 0) break;
-        s = S::STAGES;
-        --round;
-      }
-      --s;
-      ok = mbar_wait(smem_u32(&bar_empty[s]), round & 1u);
-    }
-  } else if (warp == 1) {
-    if (S::CTAS == 1 || rank == 0) {
-      int s = 0, buffer = 0;
-      uint32_t round = 0, made = 0;  // accumulators begun
+  // The eight storing warps of the wide 8-bit form need more registers than 12 warps can have alike: 128 x 56 + 256 x 224 are the
+  // 384 x 168 of the launch.
+  if (warp < FIRST_STORE_WARP) {
+    if constexpr (S::STORE_WARPS == 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      int s = 0;
+      uint32_t round = 0;
       bool ok = true;
       const bool issues = elected();
+      const uint32_t leader_full = S::CTAS == 2 ? mapped(smem_u32(bar_full), 0) : smem_u32(bar_full);
       for (int t = walker; ok && t < tiles.total; t += walkers) {
         const Tile tile = uniform(tiles.at(t, p, part, parts));
-        const uint32_t instruction = p.instruction | ((uint32_t)(tile.n >> 3) << 17);
-        uint32_t sums = 0;
+        const int mine = tile.n / S::CTAS, row = tile.row0 + (S::CTAS == 2 ? rank * mine : 0);
+        const int col = tile.col0 + (S::CTAS == 2 ? rank * LANES : 0);
+        const int boxes = (mine + S::ROW_BOX - 1) / S::ROW_BOX;
+        const uint32_t bytes = (uint32_t)(S::L_BYTES + boxes * S::ROW_BOX * ROW_BYTES);
         for (int kb = 0; kb < tile.k_blocks; ++kb) {
-          const bool fresh = S::FP8 || kb == 0;
-          if (fresh) {
-            buffer = (int)(made % S::BUFFERS);
-            if (made >= S::BUFFERS) ok = mbar_wait(smem_u32(&bar_stored[buffer]), (made / S::BUFFERS - 1) & 1u);
-            sums = tmem + (uint32_t)(buffer * S::TILE);
-            ++made;
-          }
-          ok = __all_sync(FULL, ok && mbar_wait(smem_u32(&bar_full[s]), round & 1u));
+          if (round > 0) ok = __all_sync(FULL, mbar_wait(smem_u32(&bar_empty[s]), (round - 1) & 1u));
           if (!ok) {
             if (issues) gave_up();
             break;
           }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t l = stage0 + (uint32_t)(s * S::STAGE), tt = l + S::L_BYTES;
-          const bool last = kb == tile.k_blocks - 1;
-          const int steps = S::INNER && last ? (tile.k_valid + S::MMA_STEP - 1) / S::MMA_STEP : S::STEP / S::MMA_STEP;
-          const uint64_t a = S::MN ? make_desc(l, BOX_BYTES, 1024u) : make_desc(l, 16u, 1024u);
-          const uint64_t b = S::INNER ? make_desc(tt, BOX_BYTES, 1024u) : make_desc(tt, 16u, 1024u);
-          constexpr uint64_t A_STEP = S::MN ? S::MMA_STEP * ROW_BYTES / 16 : 2, B_STEP = S::INNER ? S::MMA_STEP * ROW_BYTES / 16 : 2;
-          if (issues) {
-#pragma unroll
-            for (int k = 0; k < S::STEP / S::MMA_STEP; ++k)
-              if (!S::INNER || k < steps)
-                issue_mma<S::CTAS, S::FP8>(sums, a + (uint64_t)k * A_STEP, b + (uint64_t)k * B_STEP, instruction, k > 0 || !fresh);
-            mma_commit<S::CTAS>(smem_u32(&bar_empty[s]));
-            if (S::FP8 || last) mma_commit<S::CTAS>(smem_u32(&bar_sums[buffer]));
+          uint32_t bar = leader_full + (uint32_t)(8 * s);
+          if constexpr (S::INNER) {
+            if (kb == tile.k_blocks - 1 && tile.k_valid % S::MMA_STEP != 0) bar = smem_u32(&bar_landed[s]);
+            const int k = tile.k0 + kb * S::STEP;
+            if (issues) {
+              mbar_arrive_expect(bar, bytes);
+              tma_load_2d<S::CTAS>(l, &map_l, col, k, bar);
+              tma_load_2d<S::CTAS>(l + BOX_BYTES, &map_l, col + 64, k, bar);
+              for (int b = 0; b < boxes; ++b) tma_load_2d<S::CTAS>(tt + (uint32_t)(b * BOX_BYTES), &map_t, row + 64 * b, k, bar);
+            }
+          } else {
+            const int k = (tile.k0 + kb) * S::STEP;
+            if (issues) {
+              mbar_arrive_expect(bar, bytes);
+              if constexpr (!S::MN) {
+                tma_load_3d<S::CTAS>(l, &map_l, k, col, tile.group, bar);
+              } else {
+                tma_load_3d<S::CTAS>(l, &map_l, col, k, tile.group, bar);
+                if constexpr (!S::FP8) tma_load_3d<S::CTAS>(l + BOX_BYTES, &map_l, col + 64, k, tile.group, bar);
+              }
+              for (int b = 0; b < boxes; ++b)
+                tma_load_2d<S::CTAS>(tt + (uint32_t)(b * S::ROW_BOX * ROW_BYTES), &map_t, k, row + b * S::ROW_BOX, bar);
+            }
           }
           __syncwarp();
           if (++s == S::STAGES) { s = 0; ++round; }
         }
       }
-    }
-  } else if (warp == 2) {
-    if constexpr (S::INNER) {
-      // The last stage of a group also holds rows behind the group's last: those that an MMA would read become zeros in both
-      // operands (only one would leave a product of zero and whatever the other rows hold).
-      uint32_t used = 0, turns = 0;  // stages copied so far; a bit per stage: parity of its turns here
-      bool ok = true;
-      const uint32_t leader_full = S::CTAS == 2 ? mapped(smem_u32(bar_full), 0) : smem_u32(bar_full);
-      for (int t = walker; ok && t < tiles.total; t += walkers) {
-        const Tile tile = tiles.at(t, p, part, parts);
-        used += (uint32_t)tile.k_blocks;
-        if (tile.k_blocks == 0 || tile.k_valid % S::MMA_STEP == 0) continue;
-        const int s = (int)((used - 1) % S::STAGES);
-        ok = mbar_wait(smem_u32(&bar_landed[s]), (turns >> s) & 1u);
-        ok = __all_sync(FULL, ok);
-        if (!ok) {
-          if (lane == 0) gave_up();
-          break;
+      // the last arrivals on `empty` before the shared memory goes back
+      for (int i = 0; ok && i < S::STAGES; ++i) {
+        if (s == 0) {
+          if (round == 0) break;
+          s = S::STAGES;
+          --round;
         }
-        turns ^= 1u << s;
-        const uint32_t base = stage0 + (uint32_t)(s * S::STAGE);
-        const int clear = (tile.k_valid + S::MMA_STEP - 1) / S::MMA_STEP * S::MMA_STEP - tile.k_valid;
-        constexpr int BOXES = S::STAGE / BOX_BYTES, PIECES = ROW_BYTES / 16;
-        for (int i = lane; i < clear * BOXES * PIECES; i += 32) {
-          const int piece = i % PIECES, box = i / PIECES % BOXES, row = tile.k_valid + i / (PIECES * BOXES);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + (uint32_t)(box * BOX_BYTES + row * ROW_BYTES + piece * 16)),
-                       "r"(0u) : "memory");
+        --s;
+        ok = mbar_wait(smem_u32(&bar_empty[s]), round & 1u);
+      }
+    } else if (warp == 1) {
+      if (S::CTAS == 1 || rank == 0) {
+        int s = 0, buffer = 0;
+        uint32_t round = 0, made = 0;  // accumulators begun
+        bool ok = true;
+        const bool issues = elected();
+        for (int t = walker; ok && t < tiles.total; t += walkers) {
+          const Tile tile = uniform(tiles.at(t, p, part, parts));
+          const uint32_t instruction = p.instruction | ((uint32_t)(tile.n >> 3) << 17);
+          uint32_t sums = 0;
+          for (int kb = 0; kb < tile.k_blocks; ++kb) {
+            const bool fresh = S::FP8 || kb == 0;
+            if (fresh) {
+              buffer = (int)(made % S::BUFFERS);
+              if (made >= S::BUFFERS) ok = mbar_wait(smem_u32(&bar_stored[buffer]), (made / S::BUFFERS - 1) & 1u);
+              sums = tmem + (uint32_t)(buffer * S::TILE);
+              ++made;
+            }
+            ok = __all_sync(FULL, ok && mbar_wait(smem_u32(&bar_full[s]), round & 1u));
+            if (!ok) {
+              if (issues) gave_up();
+              break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t l = stage0 + (uint32_t)(s * S::STAGE), tt = l + S::L_BYTES;
+            const bool last = kb == tile.k_blocks - 1;
+            const int steps = S::INNER && last ? (tile.k_valid + S::MMA_STEP - 1) / S::MMA_STEP : S::STEP / S::MMA_STEP;
+            const uint64_t a = S::MN ? make_desc(l, BOX_BYTES, 1024u) : make_desc(l, 16u, 1024u);
+            const uint64_t b = S::INNER ? make_desc(tt, BOX_BYTES, 1024u) : make_desc(tt, 16u, 1024u);
+            constexpr uint64_t A_STEP = S::MN ? S::MMA_STEP * ROW_BYTES / 16 : 2, B_STEP = S::INNER ? S::MMA_STEP * ROW_BYTES / 16 : 2;
+            if (issues) {
+  #pragma unroll
+              for (int k = 0; k < S::STEP / S::MMA_STEP; ++k)
+                if (!S::INNER || k < steps)
+                  issue_mma<S::CTAS, S::FP8>(sums, a + (uint64_t)k * A_STEP, b + (uint64_t)k * B_STEP, instruction, k > 0 || !fresh);
+              mma_commit<S::CTAS>(smem_u32(&bar_empty[s]));
+              if (S::FP8 || last) mma_commit<S::CTAS>(smem_u32(&bar_sums[buffer]));
+            }
+            __syncwarp();
+            if (++s == S::STAGES) { s = 0; ++round; }
+          }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive<true>(leader_full + (uint32_t)(8 * s));
+      }
+    } else if (warp == 2) {
+      if constexpr (S::INNER) {
+        // The last stage of a group also holds rows behind the group's last: those that an MMA would read become zeros in both
+        // operands (only one would leave a product of zero and whatever the other rows hold).
+        uint32_t used = 0, turns = 0;  // stages copied so far; a bit per stage: parity of its turns here
+        bool ok = true;
+        const uint32_t leader_full = S::CTAS == 2 ? mapped(smem_u32(bar_full), 0) : smem_u32(bar_full);
+        for (int t = walker; ok && t < tiles.total; t += walkers) {
+          const Tile tile = tiles.at(t, p, part, parts);
+          used += (uint32_t)tile.k_blocks;
+          if (tile.k_blocks == 0 || tile.k_valid % S::MMA_STEP == 0) continue;
+          const int s = (int)((used - 1) % S::STAGES);
+          ok = mbar_wait(smem_u32(&bar_landed[s]), (turns >> s) & 1u);
+          ok = __all_sync(FULL, ok);
+          if (!ok) {
+            if (lane == 0) gave_up();
+            break;
+          }
+          turns ^= 1u << s;
+          const uint32_t base = stage0 + (uint32_t)(s * S::STAGE);
+          const int clear = (tile.k_valid + S::MMA_STEP - 1) / S::MMA_STEP * S::MMA_STEP - tile.k_valid;
+          constexpr int BOXES = S::STAGE / BOX_BYTES, PIECES = ROW_BYTES / 16;
+          for (int i = lane; i < clear * BOXES * PIECES; i += 32) {
+            const int piece = i % PIECES, box = i / PIECES % BOXES, row = tile.k_valid + i / (PIECES * BOXES);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + (uint32_t)(box * BOX_BYTES + row * ROW_BYTES + piece * 16)),
+                         "r"(0u) : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive<true>(leader_full + (uint32_t)(8 * s));
+        }
       }
     }
-  } else if (warp >= FIRST_STORE_WARP) {
+  } else {
+    if constexpr (S::STORE_WARPS == 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int store_warp = warp - FIRST_STORE_WARP, quarter = warp & 3;
     const int c0 = store_warp / 4 * S::WARP_COLS;  // first accumulator column of this warp
     const uint32_t lanes_at = (uint32_t)(quarter * 32) << 16;
@@ -594,21 +600,25 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
           if (kb + 1 < tile.k_blocks) fetch(kb + 1);
           const int buffer = (int)(made % S::BUFFERS);
           if (!wait_sums(buffer)) break;
+          // The loads of 32 columns run while those before are added.
+          const uint32_t at = tmem + lanes_at + (uint32_t)(buffer * S::TILE + c0);
+          uint32_t v[2][32];
+          if (c0 < tile.valid) tmem_load(v[0], at);
 #pragma unroll
           for (int c = 0; c < S::WARP_COLS; c += 32) {
+            uint32_t (&now)[32] = v[c / 32 % 2];
+            tmem_wait_loads();
+            if (c + 32 < S::WARP_COLS && c0 + c + 32 < tile.valid) tmem_load(v[(c / 32 + 1) % 2], at + (uint32_t)(c + 32));
+            if (c + 32 == S::WARP_COLS) release_sums(buffer);
             if (c0 + c < tile.valid) {
-              uint32_t v[32];
-              tmem_load(v, tmem + lanes_at + (uint32_t)(buffer * S::TILE + c0 + c));
-              tmem_wait_loads();
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
                 const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(here + c + i);
-                sum[(c + i) / 2] = fma_two(pack(v[i], v[i + 1]), f.x, sum[(c + i) / 2]);
-                sum[(c + i) / 2 + 1] = fma_two(pack(v[i + 2], v[i + 3]), f.y, sum[(c + i) / 2 + 1]);
+                sum[(c + i) / 2] = fma_two(pack(now[i], now[i + 1]), f.x, sum[(c + i) / 2]);
+                sum[(c + i) / 2 + 1] = fma_two(pack(now[i + 2], now[i + 3]), f.y, sum[(c + i) / 2 + 1]);
               }
             }
           }
-          release_sums(buffer);
         }
         if (!ok) break;
         if (S::SPLITS && parts > 1) {
