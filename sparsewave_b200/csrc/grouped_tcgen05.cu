@@ -18,6 +18,10 @@
 // Roles: warp 0 copies, warp 1 issues the MMAs, warp 2 clears the rows behind a group's last (inner form),
 // four warps (wide 8-bit: eight) from warp 4 on read the accumulators, round and store.
 //
+// Wide 8-bit tiles have their rows on the lanes and 256 columns of the weights as accumulator columns: a row's scale is then one
+// register of its lane.  (With the columns on the lanes each row's scale must reach all lanes, 128 KB a block through the
+// shared memory's 128 bytes a clock, twice the time of the block's products: 8192^3 905 us.)
+//
 // 8-bit operands: the 128 products of a scale block are one chain of the tensor core in an accumulator of its own; the storing
 // warps add it, times the scales of its row and block, to f32 sums in their registers (two sums per fma.f32x2).
 //
@@ -47,10 +51,12 @@ template <int CTAS_, int TILE_, bool FP8_, bool MN_, bool INNER_>
 struct Config {
   static constexpr int CTAS = CTAS_, TILE = TILE_;   // TILE: accumulator columns, the rows of a tile
   static constexpr bool FP8 = FP8_, MN = MN_, INNER = INNER_;  // MN: the lanes' operand has its columns contiguous
+  // 8-bit pairs have the rows on the lanes instead: see above.
+  static constexpr bool ROWS_ON_LANES = FP8 && CTAS == 2;
   static constexpr int STEP = FP8 ? 128 : 64;        // inner elements of a stage: 128 bytes
   static constexpr int MMA_STEP = FP8 ? 32 : 16;     // of an MMA
   static constexpr int ROWS_CTA = TILE / CTAS;       // of a tile's rows in one CTA's shared memory
-  static constexpr int ROW_BOX = INNER ? 64 : CTAS == 2 ? 32 : 16;  // rows of a copy
+  static constexpr int ROW_BOX = INNER ? 64 : ROWS_ON_LANES ? 128 : CTAS == 2 ? 32 : 16;  // rows of a copy
   static constexpr int L_BYTES = LANES * ROW_BYTES, T_BYTES = ROWS_CTA * ROW_BYTES, STAGE = L_BYTES + T_BYTES;
   static constexpr int BUFFERS = 512 / TILE < 4 ? 512 / TILE : 4;
   static constexpr int TMEM_COLS = BUFFERS * TILE;
@@ -59,7 +65,9 @@ struct Config {
   static constexpr int THREADS = 32 * (FIRST_STORE_WARP + STORE_WARPS);
   static constexpr bool SPLITS = CTAS == 1 && !INNER;
   static constexpr int PARTIAL = SPLITS ? TILE * LANES * 4 : 0;       // f32 sums of this CTA's share of the inner axis
-  static constexpr int SCALES = FP8 ? STORE_WARPS * 2 * WARP_COLS * 4 : 0;
+  // 8 bits: scales of the rows, or (rows on the lanes) 32 x 32 results of a warp on their way to rows of C
+  static constexpr int OUT_PITCH = 80;
+  static constexpr int SCALES = ROWS_ON_LANES ? STORE_WARPS * 32 * OUT_PITCH : FP8 ? STORE_WARPS * 2 * WARP_COLS * 4 : 0;
   static constexpr int TABLE = (int)kMaxGroups * 12 + 16;             // spans and tile counts
   static constexpr int STAGES = (232448 - 1024 - 512 - PARTIAL - SCALES - TABLE) / STAGE;
   static constexpr int SMEM = 1024 + STAGES * STAGE + PARTIAL + SCALES + TABLE;
@@ -213,8 +221,9 @@ __device__ __forceinline__ void row_tiles(int m, int tile, int round, int *count
 }
 
 struct Tile {
-  int group, row0, valid, n;  // rows [row0, row0 + valid) as accumulator columns, n of them computed (inner form: of axis i)
+  int group, row0, valid;     // rows [row0, row0 + valid) (inner form: of axis i)
   int col0;                   // first output column of this CTA (pair)
+  int n;                      // accumulator columns that are computed: those of the rows, or (rows on the lanes) of the columns
   int k0, k_blocks, k_valid;  // first stage of the inner axis, stages, elements of the last that exist
 };
 
@@ -269,7 +278,9 @@ struct Tiles {
       tile.col0 = in_band / band_rows * (LANES * S::CTAS);
       tile.row0 = span.x + row_tile * height;
       tile.valid = span.y - tile.row0 < height ? span.y - tile.row0 : height;
-      tile.n = (tile.valid + S::ROUND - 1) / S::ROUND * S::ROUND;
+      int n = tile.valid;
+      if constexpr (S::ROWS_ON_LANES) n = p.cols - tile.col0 < S::TILE ? p.cols - tile.col0 : S::TILE;
+      tile.n = (n + S::ROUND - 1) / S::ROUND * S::ROUND;
       const int blocks = (p.inner + S::STEP - 1) / S::STEP;
       tile.k0 = (int)((int64_t)blocks * part / parts);
       tile.k_blocks = (int)((int64_t)blocks * (part + 1) / parts) - tile.k0;
@@ -390,7 +401,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
         const Tile tile = uniform(tiles.at(t, p, part, parts));
         const int mine = tile.n / S::CTAS, row = tile.row0 + (S::CTAS == 2 ? rank * mine : 0);
         const int col = tile.col0 + (S::CTAS == 2 ? rank * LANES : 0);
-        const int boxes = (mine + S::ROW_BOX - 1) / S::ROW_BOX;
+        const int boxes = S::ROWS_ON_LANES ? 1 : (mine + S::ROW_BOX - 1) / S::ROW_BOX;
         const uint32_t bytes = (uint32_t)(S::L_BYTES + boxes * S::ROW_BOX * ROW_BYTES);
         for (int kb = 0; kb < tile.k_blocks; ++kb) {
           if (round > 0) ok = __all_sync(FULL, mbar_wait(smem_u32(&bar_empty[s]), (round - 1) & 1u));
@@ -413,14 +424,21 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
             const int k = (tile.k0 + kb) * S::STEP;
             if (issues) {
               mbar_arrive_expect(bar, bytes);
-              if constexpr (!S::MN) {
-                tma_load_3d<S::CTAS>(l, &map_l, k, col, tile.group, bar);
+              if constexpr (S::ROWS_ON_LANES) {  // map_l: the weights, which are the columns' operand here
+                const int w = tile.col0 + rank * mine;
+                tma_load_2d<S::CTAS>(l, &map_t, k, tile.row0 + rank * LANES, bar);
+                if constexpr (S::MN) tma_load_3d<S::CTAS>(tt, &map_l, w, k, tile.group, bar);
+                else tma_load_3d<S::CTAS>(tt, &map_l, k, w, tile.group, bar);
               } else {
-                tma_load_3d<S::CTAS>(l, &map_l, col, k, tile.group, bar);
-                if constexpr (!S::FP8) tma_load_3d<S::CTAS>(l + BOX_BYTES, &map_l, col + 64, k, tile.group, bar);
+                if constexpr (!S::MN) {
+                  tma_load_3d<S::CTAS>(l, &map_l, k, col, tile.group, bar);
+                } else {
+                  tma_load_3d<S::CTAS>(l, &map_l, col, k, tile.group, bar);
+                  if constexpr (!S::FP8) tma_load_3d<S::CTAS>(l + BOX_BYTES, &map_l, col + 64, k, tile.group, bar);
+                }
+                for (int b = 0; b < boxes; ++b)
+                  tma_load_2d<S::CTAS>(tt + (uint32_t)(b * S::ROW_BOX * ROW_BYTES), &map_t, k, row + b * S::ROW_BOX, bar);
               }
-              for (int b = 0; b < boxes; ++b)
-                tma_load_2d<S::CTAS>(tt + (uint32_t)(b * S::ROW_BOX * ROW_BYTES), &map_t, k, row + b * S::ROW_BOX, bar);
             }
           }
           __syncwarp();
@@ -464,9 +482,10 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
             const uint32_t l = stage0 + (uint32_t)(s * S::STAGE), tt = l + S::L_BYTES;
             const bool last = kb == tile.k_blocks - 1;
             const int steps = S::INNER && last ? (tile.k_valid + S::MMA_STEP - 1) / S::MMA_STEP : S::STEP / S::MMA_STEP;
-            const uint64_t a = S::MN ? make_desc(l, BOX_BYTES, 1024u) : make_desc(l, 16u, 1024u);
-            const uint64_t b = S::INNER ? make_desc(tt, BOX_BYTES, 1024u) : make_desc(tt, 16u, 1024u);
-            constexpr uint64_t A_STEP = S::MN ? S::MMA_STEP * ROW_BYTES / 16 : 2, B_STEP = S::INNER ? S::MMA_STEP * ROW_BYTES / 16 : 2;
+            constexpr bool A_MN = S::MN && !S::ROWS_ON_LANES, B_MN = S::INNER || (S::MN && S::ROWS_ON_LANES);
+            constexpr uint64_t A_STEP = A_MN ? S::MMA_STEP * ROW_BYTES / 16 : 2, B_STEP = B_MN ? S::MMA_STEP * ROW_BYTES / 16 : 2;
+            const uint64_t a = A_MN ? make_desc(l, BOX_BYTES, 1024u) : make_desc(l, 16u, 1024u);
+            const uint64_t b = B_MN ? make_desc(tt, BOX_BYTES, 1024u) : make_desc(tt, 16u, 1024u);
             if (issues) {
   #pragma unroll
               for (int k = 0; k < S::STEP / S::MMA_STEP; ++k)
@@ -538,11 +557,94 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
     };
     for (int t = walker; ok && t < tiles.total; t += walkers) {
       const Tile tile = tiles.at(t, p, part, parts);
+      if constexpr (S::ROWS_ON_LANES) {
+        const int row = tile.row0 + rank * LANES + quarter * 32 + lane, rows_end = tile.row0 + tile.valid;
+        const int used = tile.n - c0;  // accumulator columns of this warp that are computed
+        uint64_t sum[S::WARP_COLS / 2];
+#pragma unroll
+        for (int i = 0; i < S::WARP_COLS / 2; ++i) sum[i] = 0;
+        // The scales of eight blocks at a time, asked for eight blocks ahead: a load takes about as long as two blocks' products.
+        constexpr int AHEAD = 8;
+        float scale[AHEAD], next[AHEAD];
+        const bool exists = row < rows_end && used > 0;
+        const float *a_scale = p.a_scales + row;
+        const float *b_scale = p.b_scales + (int64_t)tile.group * p.scale_group + (int64_t)((tile.col0 + c0) / 128) * p.scale_j;
+        auto fetch = [&](int kb) {
+#pragma unroll
+          for (int i = 0; i < AHEAD; ++i)
+            next[i] = exists && kb + i < tile.k_blocks
+                          ? __ldg(a_scale + (int64_t)(kb + i) * p.rows) * __ldg(b_scale + (int64_t)(kb + i) * p.scale_k) : 0.0f;
+        };
+        fetch(0);
+        for (int k8 = 0; ok && k8 < tile.k_blocks; k8 += AHEAD) {
+#pragma unroll
+          for (int i = 0; i < AHEAD; ++i) scale[i] = next[i];
+          fetch(k8 + AHEAD);
+#pragma unroll
+          for (int k = 0; k < AHEAD; ++k) {
+            if (k8 + k >= tile.k_blocks) break;
+            const int buffer = (int)(made % S::BUFFERS);
+            if (!wait_sums(buffer)) break;
+            const uint32_t at = tmem + lanes_at + (uint32_t)(buffer * S::TILE + c0);
+            const uint64_t f = pack(__float_as_uint(scale[k]), __float_as_uint(scale[k]));
+            uint32_t v[2][32];  // the loads of 32 columns run while those before are added
+            if (used > 0) tmem_load(v[0], at);
+#pragma unroll
+            for (int c = 0; c < S::WARP_COLS; c += 32) {
+              uint32_t (&now)[32] = v[c / 32 % 2];
+              tmem_wait_loads();
+              if (c + 32 < S::WARP_COLS && c + 32 < used) tmem_load(v[(c / 32 + 1) % 2], at + (uint32_t)(c + 32));
+              if (c + 32 == S::WARP_COLS) release_sums(buffer);
+              if (c < used) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) sum[(c + i) / 2] = fma_two(pack(now[i], now[i + 1]), f, sum[(c + i) / 2]);
+              }
+            }
+          }
+        }
+        if (!ok) break;
+        const int cols_left = p.cols - tile.col0 - c0;
+        const bool vectors = p.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
+        uint8_t *staged = reinterpret_cast<uint8_t *>(scales) + store_warp * 32 * S::OUT_PITCH;
+#pragma unroll
+        for (int c = 0; c < S::WARP_COLS; c += 32) {
+          if (c >= cols_left) break;
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            uint32_t lo, hi;
+            unpack(sum[c / 2 + i], lo, hi);
+            w[i] = rounded(__uint_as_float(lo), false) | (uint32_t)rounded(__uint_as_float(hi), false) << 16;
+          }
+          if (vectors) {  // by way of shared memory: four lanes store 64 adjacent bytes of a row
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4 *>(staged + lane * S::OUT_PITCH + i * 16) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = i * 8 + lane / 4, piece = lane % 4;
+              const uint4 v = *reinterpret_cast<const uint4 *>(staged + r * S::OUT_PITCH + piece * 16);
+              const int to = tile.row0 + rank * LANES + quarter * 32 + r;
+              if (to < rows_end && c + piece * 8 < cols_left)
+                *reinterpret_cast<uint4 *>(p.out + (int64_t)to * p.cols + tile.col0 + c0 + c + piece * 8) = v;
+            }
+          } else if (row < rows_end) {
+            uint16_t *out = p.out + (int64_t)row * p.cols + tile.col0 + c0 + c;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c + i < cols_left) out[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
+          }
+        }
+        continue;
+      }
       const int col = tile.col0 + (S::CTAS == 2 ? rank * LANES : 0) + quarter * 32 + lane;
       const bool stores = col < p.cols;
       uint16_t *out = p.out + (S::INNER ? ((int64_t)tile.group * p.inner + tile.row0) * p.cols + col
                                         : (int64_t)tile.row0 * p.cols + col);
-      if constexpr (!S::FP8) {
+      if constexpr (S::ROWS_ON_LANES) {
+      } else if constexpr (!S::FP8) {
         if (S::INNER && tile.k_blocks == 0) {  // a group without rows
           if (stores)
             for (int c = 0; c < tile.valid; ++c) out[(int64_t)c * p.cols] = 0;
@@ -779,11 +881,13 @@ cudaError_t launch_rows(const GroupedArgs &a, Product p, int parts, const Device
   using S = Config<CTAS, TILE, FP8, MN, false>;
   CUtensorMap map_l, map_t;
   const int b_type = FP8 ? a.b_type : a.type;
+  // (rows on the lanes: boxes of 128 rows or columns of either operand)
   const bool made = (MN ? make_map(&map_l, a.B, b_type, a.n, a.inner, a.groups, S::STEP)
                         : make_map(&map_l, a.B, b_type, a.inner, a.n, a.groups, LANES)) &&
                     make_map(&map_t, a.A, a.type, a.inner, a.rows, 0, S::ROW_BOX);
   if (!made) return cudaErrorInvalidValue;
-  p.instruction = instruction_descriptor(b_type, a.type, MN, false, LANES * CTAS);
+  p.instruction = S::ROWS_ON_LANES ? instruction_descriptor(a.type, b_type, false, MN, LANES * CTAS)
+                                   : instruction_descriptor(b_type, a.type, MN, false, LANES * CTAS);
   const int64_t most = (ceil_div(a.rows, TILE) + (a.groups < a.rows ? a.groups : a.rows)) * ceil_div(a.n, LANES * CTAS);
   return launch<S>(map_l, map_t, p, most, parts, dev.sm_count, s);
 }
