@@ -67,7 +67,7 @@ struct Config {
   static constexpr int PARTIAL = SPLITS ? TILE * LANES * 4 : 0;       // f32 sums of this CTA's share of the inner axis
   // 8 bits: scales of the rows, or (rows on the lanes) 32 x 32 results of a warp on their way to rows of C
   static constexpr int OUT_PITCH = 80;
-  static constexpr int SCALES = ROWS_ON_LANES ? STORE_WARPS * 32 * OUT_PITCH : FP8 ? STORE_WARPS * 2 * WARP_COLS * 4 : 0;
+  static constexpr int SCALES = ROWS_ON_LANES ? STORE_WARPS * 32 * OUT_PITCH : FP8 ? STORE_WARPS * 4 * WARP_COLS * 4 : 0;
   static constexpr int TABLE = (int)kMaxGroups * 12 + 16;             // spans and tile counts
   static constexpr int STAGES = (232448 - 1024 - 512 - PARTIAL - SCALES - TABLE) / STAGE;
   static constexpr int SMEM = 1024 + STAGES * STAGE + PARTIAL + SCALES + TABLE;
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   const uint32_t stage0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t *behind = smem_raw + (stage0 - smem_u32(smem_raw)) + S::STAGES * S::STAGE;
   float *partial = reinterpret_cast<float *>(behind);                         // [TILE][LANES]
-  float *scales = reinterpret_cast<float *>(behind + S::PARTIAL);             // [warp][2][WARP_COLS]
+  float *scales = reinterpret_cast<float *>(behind + S::PARTIAL);             // [warp][4][WARP_COLS]
   int2 *spans = reinterpret_cast<int2 *>(behind + S::PARTIAL + S::SCALES);
   int *first = reinterpret_cast<int *>(spans + kMaxGroups);
   const int rank = S::CTAS == 2 || S::SPLITS ? (int)(blockIdx.x % (unsigned)(S::CTAS == 2 ? 2 : parts)) : 0;
@@ -467,13 +467,14 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
           uint32_t sums = 0;
           for (int kb = 0; kb < tile.k_blocks; ++kb) {
             const bool fresh = S::FP8 || kb == 0;
+            ok = mbar_wait(smem_u32(&bar_full[s]), round & 1u);
             if (fresh) {
               buffer = (int)(made % S::BUFFERS);
-              if (made >= S::BUFFERS) ok = mbar_wait(smem_u32(&bar_stored[buffer]), (made / S::BUFFERS - 1) & 1u);
+              if (made >= S::BUFFERS) ok = ok && mbar_wait(smem_u32(&bar_stored[buffer]), (made / S::BUFFERS - 1) & 1u);
               sums = tmem + (uint32_t)(buffer * S::TILE);
               ++made;
             }
-            ok = __all_sync(FULL, ok && mbar_wait(smem_u32(&bar_full[s]), round & 1u));
+            ok = __all_sync(FULL, ok);
             if (!ok) {
               if (issues) gave_up();
               break;
@@ -487,7 +488,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
             const uint64_t a = A_MN ? make_desc(l, BOX_BYTES, 1024u) : make_desc(l, 16u, 1024u);
             const uint64_t b = B_MN ? make_desc(tt, BOX_BYTES, 1024u) : make_desc(tt, 16u, 1024u);
             if (issues) {
-  #pragma unroll
+#pragma unroll
               for (int k = 0; k < S::STEP / S::MMA_STEP; ++k)
                 if (!S::INNER || k < steps)
                   issue_mma<S::CTAS, S::FP8>(sums, a + (uint64_t)k * A_STEP, b + (uint64_t)k * B_STEP, instruction, k > 0 || !fresh);
@@ -563,26 +564,29 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
         uint64_t sum[S::WARP_COLS / 2];
 #pragma unroll
         for (int i = 0; i < S::WARP_COLS / 2; ++i) sum[i] = 0;
-        // The scales of eight blocks at a time, asked for eight blocks ahead: a load takes about as long as two blocks' products.
-        constexpr int AHEAD = 8;
-        float scale[AHEAD], next[AHEAD];
-        const bool exists = row < rows_end && used > 0;
-        const float *a_scale = p.a_scales + row;
-        const float *b_scale = p.b_scales + (int64_t)tile.group * p.scale_group + (int64_t)((tile.col0 + c0) / 128) * p.scale_j;
+        // The scales of four blocks at a time, asked for four blocks ahead.  Loads of places that exist, whatever the lane's row: behind
+        // a condition each would wait for the one before (eight loads some 7,000 clocks).
+        constexpr int AHEAD = 4;
+        float scale[AHEAD], next_a[AHEAD], next_b[AHEAD];
+        const float *a_scale = p.a_scales + (row < rows_end ? row : tile.row0);
+        const float *b_scale = p.b_scales + (int64_t)tile.group * p.scale_group +
+                               (int64_t)((tile.col0 + (used > 0 ? c0 : 0)) / 128) * p.scale_j;
         auto fetch = [&](int kb) {
 #pragma unroll
-          for (int i = 0; i < AHEAD; ++i)
-            next[i] = exists && kb + i < tile.k_blocks
-                          ? __ldg(a_scale + (int64_t)(kb + i) * p.rows) * __ldg(b_scale + (int64_t)(kb + i) * p.scale_k) : 0.0f;
+          for (int i = 0; i < AHEAD; ++i) {
+            const int64_t block = kb + i < tile.k_blocks ? kb + i : tile.k_blocks - 1;
+            next_a[i] = __ldg(a_scale + block * p.rows);
+            next_b[i] = __ldg(b_scale + block * p.scale_k);
+          }
         };
         fetch(0);
-        for (int k8 = 0; ok && k8 < tile.k_blocks; k8 += AHEAD) {
+        for (int k4 = 0; ok && k4 < tile.k_blocks; k4 += AHEAD) {
 #pragma unroll
-          for (int i = 0; i < AHEAD; ++i) scale[i] = next[i];
-          fetch(k8 + AHEAD);
+          for (int i = 0; i < AHEAD; ++i) scale[i] = next_a[i] * next_b[i];
+          fetch(k4 + AHEAD);
 #pragma unroll
           for (int k = 0; k < AHEAD; ++k) {
-            if (k8 + k >= tile.k_blocks) break;
+            if (k4 + k >= tile.k_blocks) break;
             const int buffer = (int)(made % S::BUFFERS);
             if (!wait_sums(buffer)) break;
             const uint32_t at = tmem + lanes_at + (uint32_t)(buffer * S::TILE + c0);
@@ -678,46 +682,53 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
         uint64_t sum[S::WARP_COLS / 2];
 #pragma unroll
         for (int i = 0; i < S::WARP_COLS / 2; ++i) sum[i] = 0;
-        float *mine = scales + store_warp * 2 * S::WARP_COLS;
+        float *mine = scales + store_warp * 4 * S::WARP_COLS;
         const float *b_scale = p.b_scales + (int64_t)tile.group * p.scale_group +
-                               (int64_t)((tile.col0 + (S::CTAS == 2 ? rank * LANES : 0)) / 128) * p.scale_j;
-        const bool any_col = tile.col0 + (S::CTAS == 2 ? rank * LANES : 0) < p.cols;
-        constexpr int PER_LANE = S::WARP_COLS / 32;
-        float next[PER_LANE];
-        auto fetch = [&](int kb) {
-          const int64_t block = tile.k0 + kb;
-          const float sb = any_col ? __ldg(b_scale + block * p.scale_k) : 0.0f;
+                               (int64_t)(tile.col0 / 128) * p.scale_j;
+        constexpr int PER_LANE = S::WARP_COLS / 32, AHEAD = 4;
+        float next_a[AHEAD][PER_LANE], next_b[AHEAD];
+        auto fetch = [&](int kb) {  // four blocks' scales, of rows that exist (see above)
 #pragma unroll
-          for (int i = 0; i < PER_LANE; ++i) {
-            const int c = c0 + i * 32 + lane;
-            next[i] = c < tile.valid ? sb * __ldg(p.a_scales + block * p.rows + tile.row0 + c) : 0.0f;
+          for (int j = 0; j < AHEAD; ++j) {
+            const int64_t block = tile.k0 + (kb + j < tile.k_blocks ? kb + j : tile.k_blocks - 1);
+            next_b[j] = __ldg(b_scale + block * p.scale_k);
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i) {
+              const int c = c0 + i * 32 + lane;
+              next_a[j][i] = __ldg(p.a_scales + block * p.rows + tile.row0 + (c < tile.valid ? c : 0));
+            }
           }
         };
         if (tile.k_blocks > 0) fetch(0);
-        for (int kb = 0; kb < tile.k_blocks; ++kb) {
-          float *here = mine + (kb & 1) * S::WARP_COLS;
-#pragma unroll
-          for (int i = 0; i < PER_LANE; ++i) here[i * 32 + lane] = next[i];
+        for (int k4 = 0; ok && k4 < tile.k_blocks; k4 += AHEAD) {
           __syncwarp();
-          if (kb + 1 < tile.k_blocks) fetch(kb + 1);
-          const int buffer = (int)(made % S::BUFFERS);
-          if (!wait_sums(buffer)) break;
-          // The loads of 32 columns run while those before are added.
-          const uint32_t at = tmem + lanes_at + (uint32_t)(buffer * S::TILE + c0);
-          uint32_t v[2][32];
-          if (c0 < tile.valid) tmem_load(v[0], at);
 #pragma unroll
-          for (int c = 0; c < S::WARP_COLS; c += 32) {
-            uint32_t (&now)[32] = v[c / 32 % 2];
-            tmem_wait_loads();
-            if (c + 32 < S::WARP_COLS && c0 + c + 32 < tile.valid) tmem_load(v[(c / 32 + 1) % 2], at + (uint32_t)(c + 32));
-            if (c + 32 == S::WARP_COLS) release_sums(buffer);
-            if (c0 + c < tile.valid) {
+          for (int j = 0; j < AHEAD; ++j)
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(here + c + i);
-                sum[(c + i) / 2] = fma_two(pack(now[i], now[i + 1]), f.x, sum[(c + i) / 2]);
-                sum[(c + i) / 2 + 1] = fma_two(pack(now[i + 2], now[i + 3]), f.y, sum[(c + i) / 2 + 1]);
+            for (int i = 0; i < PER_LANE; ++i) mine[j * S::WARP_COLS + i * 32 + lane] = next_a[j][i] * next_b[j];
+          __syncwarp();
+          fetch(k4 + AHEAD);
+          for (int k = 0; k < AHEAD && k4 + k < tile.k_blocks; ++k) {
+            const float *here = mine + k * S::WARP_COLS;
+            const int buffer = (int)(made % S::BUFFERS);
+            if (!wait_sums(buffer)) break;
+            // The loads of 32 columns run while those before are added.
+            const uint32_t at = tmem + lanes_at + (uint32_t)(buffer * S::TILE + c0);
+            uint32_t v[2][32];
+            if (c0 < tile.valid) tmem_load(v[0], at);
+#pragma unroll
+            for (int c = 0; c < S::WARP_COLS; c += 32) {
+              uint32_t (&now)[32] = v[c / 32 % 2];
+              tmem_wait_loads();
+              if (c + 32 < S::WARP_COLS && c0 + c + 32 < tile.valid) tmem_load(v[(c / 32 + 1) % 2], at + (uint32_t)(c + 32));
+              if (c + 32 == S::WARP_COLS) release_sums(buffer);
+              if (c0 + c < tile.valid) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                  const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(here + c + i);
+                  sum[(c + i) / 2] = fma_two(pack(now[i], now[i + 1]), f.x, sum[(c + i) / 2]);
+                  sum[(c + i) / 2 + 1] = fma_two(pack(now[i + 2], now[i + 3]), f.y, sum[(c + i) / 2 + 1]);
+                }
               }
             }
           }
