@@ -18,7 +18,8 @@
 // Roles: warp 0 copies, warp 1 issues the MMAs, warp 2 clears the rows behind a group's last (inner form),
 // four warps (wide 8-bit: eight) from warp 4 on read the accumulators, round and store.
 //
-// Wide 8-bit tiles have their rows on the lanes and 256 columns of the weights as accumulator columns: a row's scale is then one
+// The inner form has rows of the result on the lanes, whose results then lie in a row in each lane's registers.  Wide 8-bit tiles
+// have their rows on the lanes too, and 256 columns of the weights as accumulator columns: a row's scale is then one
 // register of its lane.  (With the columns on the lanes each row's scale must reach all lanes, 128 KB a block through the
 // shared memory's 128 bytes a clock, twice the time of the block's products: 8192^3 905 us.)
 //
@@ -51,12 +52,11 @@ template <int CTAS_, int TILE_, bool FP8_, bool MN_, bool INNER_>
 struct Config {
   static constexpr int CTAS = CTAS_, TILE = TILE_;   // TILE: accumulator columns, the rows of a tile
   static constexpr bool FP8 = FP8_, MN = MN_, INNER = INNER_;  // MN: the lanes' operand has its columns contiguous
-  // 8-bit pairs have the rows on the lanes instead: see above.
-  static constexpr bool ROWS_ON_LANES = FP8 && CTAS == 2;
+  static constexpr bool ROWS_ON_LANES = (FP8 && CTAS == 2) || INNER;  // see above
   static constexpr int STEP = FP8 ? 128 : 64;        // inner elements of a stage: 128 bytes
   static constexpr int MMA_STEP = FP8 ? 32 : 16;     // of an MMA
   static constexpr int ROWS_CTA = TILE / CTAS;       // of a tile's rows in one CTA's shared memory
-  static constexpr int ROW_BOX = INNER ? 64 : ROWS_ON_LANES ? 128 : CTAS == 2 ? 32 : 16;  // rows of a copy
+  static constexpr int ROW_BOX = INNER ? 64 : FP8 && CTAS == 2 ? 128 : CTAS == 2 ? 32 : 16;  // rows of a copy
   static constexpr int L_BYTES = LANES * ROW_BYTES, T_BYTES = ROWS_CTA * ROW_BYTES, STAGE = L_BYTES + T_BYTES;
   static constexpr int BUFFERS = 512 / TILE < 4 ? 512 / TILE : 4;
   static constexpr int TMEM_COLS = BUFFERS * TILE;
@@ -65,12 +65,12 @@ struct Config {
   static constexpr int THREADS = 32 * (FIRST_STORE_WARP + STORE_WARPS);
   static constexpr bool SPLITS = CTAS == 1 && !INNER;
   static constexpr int PARTIAL = SPLITS ? TILE * LANES * 4 : 0;       // f32 sums of this CTA's share of the inner axis
-  // 8 bits: scales of the rows, or (rows on the lanes) 32 x 32 results of a warp on their way to rows of C
-  static constexpr int OUT_PITCH = 80;
-  static constexpr int SCALES = ROWS_ON_LANES ? STORE_WARPS * 32 * OUT_PITCH : FP8 ? STORE_WARPS * 4 * WARP_COLS * 4 : 0;
+  static constexpr int SCALES = FP8 && !ROWS_ON_LANES ? STORE_WARPS * 4 * WARP_COLS * 4 : 0;
+  static constexpr int OUT_PITCH = 80;                                // 32 x 32 results of a warp on their way to rows of C
+  static constexpr int STAGED = STORE_WARPS * 32 * OUT_PITCH;
   static constexpr int TABLE = (int)kMaxGroups * 12 + 16;             // spans and tile counts
-  static constexpr int STAGES = (232448 - 1024 - 512 - PARTIAL - SCALES - TABLE) / STAGE;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + PARTIAL + SCALES + TABLE;
+  static constexpr int STAGES = (232448 - 1024 - 512 - PARTIAL - SCALES - STAGED - TABLE) / STAGE;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + PARTIAL + SCALES + STAGED + TABLE;
   static constexpr int ROUND = 16 * CTAS;                             // N of an MMA is a multiple of this
 };
 
@@ -194,6 +194,14 @@ __device__ __forceinline__ void tmem_load(uint32_t (&v)[32], uint32_t addr) {
         "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(addr) : "memory");
 }
+// 16 lanes x 32 accumulator columns: register 4 i + 2 a + b of lane l is lane l / 4 + 8 a, column 8 i + 2 (l % 4) + b.
+__device__ __forceinline__ void tmem_load_blocks(uint32_t (&v)[16], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(addr) : "memory");
+}
 __device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ uint64_t pack(uint32_t lo, uint32_t hi) {
@@ -212,6 +220,18 @@ __device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) 
 
 __device__ __forceinline__ uint16_t rounded(float v, bool half_out) {  // once, to nearest
   return half_out ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+
+__device__ __forceinline__ uint32_t rounded_two(float lo, float hi, bool half_out) {
+  uint32_t r;
+  if (half_out) {
+    const __half2 two = __floats2half2_rn(lo, hi);
+    memcpy(&r, &two, 4);
+  } else {
+    const __nv_bfloat162 two = __floats2bfloat162_rn(lo, hi);
+    memcpy(&r, &two, 4);
+  }
+  return r;
 }
 
 // Row tiles of a group of m rows: as few as the tile size allows, of equal heights but for the last.
@@ -255,7 +275,8 @@ struct Tiles {
       tile.col0 = local / inner_tiles * (LANES * S::CTAS);
       tile.row0 = it * S::TILE;
       tile.valid = p.inner - tile.row0 < S::TILE ? p.inner - tile.row0 : S::TILE;
-      tile.n = (tile.valid + S::ROUND - 1) / S::ROUND * S::ROUND;
+      const int n = p.cols - tile.col0 < S::TILE ? p.cols - tile.col0 : S::TILE;
+      tile.n = (n + S::ROUND - 1) / S::ROUND * S::ROUND;
       const int2 span = spans[tile.group];
       const int m = span.y - span.x;
       tile.k0 = span.x;
@@ -305,7 +326,8 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   uint8_t *behind = smem_raw + (stage0 - smem_u32(smem_raw)) + S::STAGES * S::STAGE;
   float *partial = reinterpret_cast<float *>(behind);                         // [TILE][LANES]
   float *scales = reinterpret_cast<float *>(behind + S::PARTIAL);             // [warp][4][WARP_COLS]
-  int2 *spans = reinterpret_cast<int2 *>(behind + S::PARTIAL + S::SCALES);
+  uint8_t *staged_all = behind + S::PARTIAL + S::SCALES;
+  int2 *spans = reinterpret_cast<int2 *>(staged_all + S::STAGED);
   int *first = reinterpret_cast<int *>(spans + kMaxGroups);
   const int rank = S::CTAS == 2 || S::SPLITS ? (int)(blockIdx.x % (unsigned)(S::CTAS == 2 ? 2 : parts)) : 0;
   const int part = S::CTAS == 2 ? 0 : rank;  // of the inner axis
@@ -401,7 +423,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
         const Tile tile = uniform(tiles.at(t, p, part, parts));
         const int mine = tile.n / S::CTAS, row = tile.row0 + (S::CTAS == 2 ? rank * mine : 0);
         const int col = tile.col0 + (S::CTAS == 2 ? rank * LANES : 0);
-        const int boxes = S::ROWS_ON_LANES ? 1 : (mine + S::ROW_BOX - 1) / S::ROW_BOX;
+        const int boxes = S::FP8 && S::ROWS_ON_LANES ? 1 : (mine + S::ROW_BOX - 1) / S::ROW_BOX;
         const uint32_t bytes = (uint32_t)(S::L_BYTES + boxes * S::ROW_BOX * ROW_BYTES);
         for (int kb = 0; kb < tile.k_blocks; ++kb) {
           if (round > 0) ok = __all_sync(FULL, mbar_wait(smem_u32(&bar_empty[s]), (round - 1) & 1u));
@@ -415,10 +437,11 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
             if (kb == tile.k_blocks - 1 && tile.k_valid % S::MMA_STEP != 0) bar = smem_u32(&bar_landed[s]);
             const int k = tile.k0 + kb * S::STEP;
             if (issues) {
+              const int i = tile.row0 + rank * LANES, j = tile.col0 + rank * mine;
               mbar_arrive_expect(bar, bytes);
-              tma_load_2d<S::CTAS>(l, &map_l, col, k, bar);
-              tma_load_2d<S::CTAS>(l + BOX_BYTES, &map_l, col + 64, k, bar);
-              for (int b = 0; b < boxes; ++b) tma_load_2d<S::CTAS>(tt + (uint32_t)(b * BOX_BYTES), &map_t, row + 64 * b, k, bar);
+              tma_load_2d<S::CTAS>(l, &map_t, i, k, bar);
+              tma_load_2d<S::CTAS>(l + BOX_BYTES, &map_t, i + 64, k, bar);
+              for (int b = 0; b < boxes; ++b) tma_load_2d<S::CTAS>(tt + (uint32_t)(b * BOX_BYTES), &map_l, j + 64 * b, k, bar);
             }
           } else {
             const int k = (tile.k0 + kb) * S::STEP;
@@ -483,7 +506,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
             const uint32_t l = stage0 + (uint32_t)(s * S::STAGE), tt = l + S::L_BYTES;
             const bool last = kb == tile.k_blocks - 1;
             const int steps = S::INNER && last ? (tile.k_valid + S::MMA_STEP - 1) / S::MMA_STEP : S::STEP / S::MMA_STEP;
-            constexpr bool A_MN = S::MN && !S::ROWS_ON_LANES, B_MN = S::INNER || (S::MN && S::ROWS_ON_LANES);
+            constexpr bool A_MN = S::INNER || (S::MN && !S::ROWS_ON_LANES), B_MN = S::INNER || (S::MN && S::ROWS_ON_LANES);
             constexpr uint64_t A_STEP = A_MN ? S::MMA_STEP * ROW_BYTES / 16 : 2, B_STEP = B_MN ? S::MMA_STEP * ROW_BYTES / 16 : 2;
             const uint64_t a = A_MN ? make_desc(l, BOX_BYTES, 1024u) : make_desc(l, 16u, 1024u);
             const uint64_t b = B_MN ? make_desc(tt, BOX_BYTES, 1024u) : make_desc(tt, 16u, 1024u);
@@ -556,9 +579,54 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
       }
       ++made;
     };
+    // 32 x 32 results of the warp go to rows of C by way of shared memory: four lanes store 64 adjacent bytes of a row.
+    uint8_t *staged = staged_all + store_warp * 32 * S::OUT_PITCH;
+    const bool vectors = p.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
+    auto lay_down = [&](const uint32_t (&w)[16]) {  // the lane's row
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint4 *>(staged + lane * S::OUT_PITCH + i * 16) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    };
+    auto store_block = [&](uint16_t *out, int row0, int rows_end, int col0) {
+      __syncwarp();
+      if (vectors) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 8 + lane / 4, piece = lane % 4;
+          const uint4 v = *reinterpret_cast<const uint4 *>(staged + r * S::OUT_PITCH + piece * 16);
+          if (row0 + r < rows_end && col0 + piece * 8 < p.cols)
+            *reinterpret_cast<uint4 *>(out + (int64_t)(row0 + r) * p.cols + col0 + piece * 8) = v;
+        }
+      } else if (col0 + lane < p.cols) {
+        const int count = rows_end - row0 < 32 ? rows_end - row0 : 32;
+        for (int r = 0; r < count; ++r)
+          out[(int64_t)(row0 + r) * p.cols + col0 + lane] = *reinterpret_cast<const uint16_t *>(staged + r * S::OUT_PITCH + lane * 2);
+      }
+    };
     for (int t = walker; ok && t < tiles.total; t += walkers) {
       const Tile tile = tiles.at(t, p, part, parts);
-      if constexpr (S::ROWS_ON_LANES) {
+      if constexpr (S::INNER) {
+        const int buffer = (int)(made % S::BUFFERS);
+        const bool empty = tile.k_blocks == 0;  // a group without rows: zeros
+        if (!empty && !wait_sums(buffer)) break;
+        uint16_t *out = p.out + (int64_t)tile.group * p.inner * p.cols;
+        for (int c = 0; c < tile.n; c += 32) {
+          uint32_t v[32], w[16];
+          if (!empty) {
+            tmem_load(v, tmem + lanes_at + (uint32_t)(buffer * S::TILE + c));
+            tmem_wait_loads();
+            if (c + 32 >= tile.n) release_sums(buffer);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            w[i] = empty ? 0u : rounded_two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), p.half_out);
+          lay_down(w);
+          store_block(out, tile.row0 + rank * LANES + quarter * 32, tile.row0 + tile.valid, tile.col0 + c);
+        }
+        continue;
+      }
+      if constexpr (S::FP8 && S::ROWS_ON_LANES) {
         const int row = tile.row0 + rank * LANES + quarter * 32 + lane, rows_end = tile.row0 + tile.valid;
         const int used = tile.n - c0;  // accumulator columns of this warp that are computed
         uint64_t sum[S::WARP_COLS / 2];
@@ -607,53 +675,26 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
           }
         }
         if (!ok) break;
-        const int cols_left = p.cols - tile.col0 - c0;
-        const bool vectors = p.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
-        uint8_t *staged = reinterpret_cast<uint8_t *>(scales) + store_warp * 32 * S::OUT_PITCH;
 #pragma unroll
         for (int c = 0; c < S::WARP_COLS; c += 32) {
-          if (c >= cols_left) break;
+          if (tile.col0 + c0 + c >= p.cols) break;
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             uint32_t lo, hi;
             unpack(sum[c / 2 + i], lo, hi);
-            w[i] = rounded(__uint_as_float(lo), false) | (uint32_t)rounded(__uint_as_float(hi), false) << 16;
+            w[i] = rounded_two(__uint_as_float(lo), __uint_as_float(hi), false);
           }
-          if (vectors) {  // by way of shared memory: four lanes store 64 adjacent bytes of a row
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<uint4 *>(staged + lane * S::OUT_PITCH + i * 16) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = i * 8 + lane / 4, piece = lane % 4;
-              const uint4 v = *reinterpret_cast<const uint4 *>(staged + r * S::OUT_PITCH + piece * 16);
-              const int to = tile.row0 + rank * LANES + quarter * 32 + r;
-              if (to < rows_end && c + piece * 8 < cols_left)
-                *reinterpret_cast<uint4 *>(p.out + (int64_t)to * p.cols + tile.col0 + c0 + c + piece * 8) = v;
-            }
-          } else if (row < rows_end) {
-            uint16_t *out = p.out + (int64_t)row * p.cols + tile.col0 + c0 + c;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c + i < cols_left) out[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
-          }
+          lay_down(w);
+          store_block(p.out, tile.row0 + rank * LANES + quarter * 32, rows_end, tile.col0 + c0 + c);
         }
         continue;
       }
       const int col = tile.col0 + (S::CTAS == 2 ? rank * LANES : 0) + quarter * 32 + lane;
       const bool stores = col < p.cols;
-      uint16_t *out = p.out + (S::INNER ? ((int64_t)tile.group * p.inner + tile.row0) * p.cols + col
-                                        : (int64_t)tile.row0 * p.cols + col);
+      uint16_t *out = p.out + (int64_t)tile.row0 * p.cols + col;
       if constexpr (S::ROWS_ON_LANES) {
       } else if constexpr (!S::FP8) {
-        if (S::INNER && tile.k_blocks == 0) {  // a group without rows
-          if (stores)
-            for (int c = 0; c < tile.valid; ++c) out[(int64_t)c * p.cols] = 0;
-          continue;
-        }
         const int buffer = (int)(made % S::BUFFERS);
         if (!wait_sums(buffer)) break;
         const bool split = S::SPLITS && parts > 1;
@@ -665,18 +706,40 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
           }
         }
         for (int c = 0; c < tile.valid; c += 32) {
-          uint32_t v[32];
-          tmem_load(v, tmem + lanes_at + (uint32_t)(buffer * S::TILE + c));
-          tmem_wait_loads();
-          if (c + 32 >= tile.valid) release_sums(buffer);
+          const uint32_t at = tmem + lanes_at + (uint32_t)(buffer * S::TILE + c);
           if (split) {
+            uint32_t v[32];
+            tmem_load(v, at);
+            tmem_wait_loads();
+            if (c + 32 >= tile.valid) release_sums(buffer);
 #pragma unroll
             for (int i = 0; i < 32; ++i) partial[(c + i) * LANES + quarter * 32 + lane] = __uint_as_float(v[i]);
-          } else if (stores) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c + i < tile.valid) out[(int64_t)(c + i) * p.cols] = rounded(__uint_as_float(v[i]), p.half_out);
+            continue;
           }
+          // 16 lanes x 32 columns each: blocks of 8 lanes (columns of C) x 8 columns (rows of C) as the warp-level MMAs hold them,
+          // two rows of C to a register, which stmatrix lays down transposed
+          uint32_t v[2][16];
+          tmem_load_blocks(v[0], at);
+          tmem_load_blocks(v[1], at + (16u << 16));
+          tmem_wait_loads();
+          if (c + 32 >= tile.valid) release_sums(buffer);
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              uint32_t w[4];
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+                const int r = 4 * (i + m / 2) + 2 * (m % 2);
+                w[m] = rounded_two(__uint_as_float(v[h][r]), __uint_as_float(v[h][r + 1]), p.half_out);
+              }
+              const int m = lane / 8;
+              const uint32_t to = smem_u32(staged) + (uint32_t)((8 * (i + m / 2) + lane % 8) * S::OUT_PITCH + (h * 16 + m % 2 * 8) * 2);
+              asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]),
+                           "r"(w[2]), "r"(w[3]) : "memory");
+            }
+          store_block(p.out, tile.row0 + c, tile.row0 + tile.valid, tile.col0 + (S::CTAS == 2 ? rank * LANES : 0) + quarter * 32);
         }
       } else {
         uint64_t sum[S::WARP_COLS / 2];
