@@ -15,6 +15,10 @@
 // Which tile lies where is worked out on the device from the offsets: every CTA builds the table of the groups' tiles in shared
 // memory, and the CTAs (pairs, clusters) walk the tiles in turn.
 //
+// Operands whose rows do not lie on 16-byte boundaries, which TMA cannot copy, are first copied to rows that do, in memory from the
+// context's stream-ordered pool: of the weights those of groups with rows.  (3,001 rows, 7 groups, 1111 x 777: warps that read such
+// rows themselves and shift them into place for every tile took 62 us, the copy and the product 24.)
+//
 // Roles: warp 0 copies, warp 1 issues the MMAs, warp 2 clears the rows behind a group's last (inner form),
 // four warps (wide 8-bit: eight) from warp 4 on read the accumulators, round and store.
 //
@@ -81,7 +85,8 @@ struct Product {
   uint32_t instruction;           // descriptor without N
   bool half_out;
   const float *a_scales, *b_scales;
-  int scale_k, scale_j, scale_group;
+  int scale_k, scale_j;
+  int64_t scale_group;
   int *status;
 };
 
@@ -637,7 +642,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
         constexpr int AHEAD = 4;
         float scale[AHEAD], next_a[AHEAD], next_b[AHEAD];
         const float *a_scale = p.a_scales + (row < rows_end ? row : tile.row0);
-        const float *b_scale = p.b_scales + (int64_t)tile.group * p.scale_group +
+        const float *b_scale = p.b_scales + tile.group * p.scale_group +
                                (int64_t)((tile.col0 + (used > 0 ? c0 : 0)) / 128) * p.scale_j;
         auto fetch = [&](int kb) {
 #pragma unroll
@@ -746,7 +751,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
 #pragma unroll
         for (int i = 0; i < S::WARP_COLS / 2; ++i) sum[i] = 0;
         float *mine = scales + store_warp * 4 * S::WARP_COLS;
-        const float *b_scale = p.b_scales + (int64_t)tile.group * p.scale_group +
+        const float *b_scale = p.b_scales + tile.group * p.scale_group +
                                (int64_t)(tile.col0 / 128) * p.scale_j;
         constexpr int PER_LANE = S::WARP_COLS / 32, AHEAD = 4;
         float next_a[AHEAD][PER_LANE], next_b[AHEAD];
@@ -870,6 +875,8 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   }
 }
 
+int64_t element_size(int type) { return type == kBF16 || type == kF16 ? 2 : 1; }
+
 using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                    const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -885,13 +892,15 @@ EncodeTiledFn encode_tiled_fn() {
   return fn;
 }
 
-// `stack` matrices of `outer` rows of `inner` contiguous elements (rank 2 without a stack), boxes of 128 swizzled bytes x box_rows.
-bool make_map(CUtensorMap *map, const void *base, int type, int64_t inner, int64_t outer, int64_t stack, uint32_t box_rows) {
+// `stack` matrices of `outer` rows of `inner` contiguous elements (rank 2 without a stack), `pitch` elements apart; boxes of 128
+// swizzled bytes x box_rows.
+bool make_map(CUtensorMap *map, const void *base, int type, int64_t inner, int64_t outer, int64_t stack, int64_t pitch,
+              uint32_t box_rows) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return false;
-  const cuuint64_t size = type == kBF16 || type == kF16 ? 2 : 1;
+  const cuuint64_t size = element_size(type);
   cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)stack};
-  cuuint64_t strides[2] = {(cuuint64_t)inner * size, (cuuint64_t)(inner * outer) * size};
+  cuuint64_t strides[2] = {(cuuint64_t)pitch * size, (cuuint64_t)(pitch * outer) * size};
   cuuint32_t box[3] = {(cuuint32_t)(ROW_BYTES / size), box_rows, 1};
   cuuint32_t elem[3] = {1, 1, 1};
   const CUtensorMapDataType data = type == kBF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
@@ -900,6 +909,118 @@ bool make_map(CUtensorMap *map, const void *base, int type, int64_t inner, int64
   return fn(map, data, stack > 0 ? 3 : 2, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+
+// A matrix (or stack of them) on its way to rows on 16-byte boundaries.
+struct Realigned {
+  const uint8_t *from;
+  uint8_t *to;           // NULL: stays where it is
+  int64_t rows;          // of all matrices
+  int64_t bytes, pitch;  // of a row; of a row of the copy
+  int64_t group_rows;    // rows of a group's matrix, of which only groups with rows are copied; 0: all
+};
+
+constexpr int REALIGN_THREADS = 256, REALIGN_AHEAD = 4;
+
+// A warp copies a row, 16 bytes of the copy a lane: aligned words of the operand shifted into place.  The first and the last bytes of
+// the operand, whose words reach over it, go byte by byte.  Bytes of the copy behind a row's last are not written (copies by
+// TMA end there).
+__global__ void __launch_bounds__(REALIGN_THREADS) realign_kernel(const Realigned a, const Realigned b, const int32_t *offsets, int rows) {
+  after_previous_kernel();
+  const int lane = threadIdx.x % 32;
+  const int64_t first = (int64_t)blockIdx.x * (REALIGN_THREADS / 32) + threadIdx.x / 32, step = (int64_t)gridDim.x * (REALIGN_THREADS / 32);
+  for (int64_t at = first; at < a.rows + b.rows; at += step) {
+    const bool second = at >= a.rows;
+    const Realigned &m = second ? b : a;
+    const int64_t row = second ? at - a.rows : at;
+    if (!m.to) continue;
+    if (m.group_rows > 0) {
+      const RowSpan span = group_rows(offsets, (int)(row / m.group_rows), rows);
+      if (span.begin == span.end) continue;
+    }
+    const uint8_t *from = m.from + row * m.bytes, *end = m.from + m.rows * m.bytes;
+    const int shift = (int)(reinterpret_cast<uintptr_t>(from) & 3u);
+    uint4 *to = reinterpret_cast<uint4 *>(m.to + row * m.pitch);
+    const int64_t pieces = (m.bytes + 15) / 16;
+    for (int64_t q0 = lane; q0 < pieces; q0 += 32 * REALIGN_AHEAD) {
+      uint32_t w[REALIGN_AHEAD][5];
+#pragma unroll
+      for (int u = 0; u < REALIGN_AHEAD; ++u) {
+        const uint8_t *p = from + (q0 + 32 * u) * 16 - shift;
+        const bool whole = q0 + 32 * u < pieces && p >= m.from && p + 20 <= end;
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[u][i] = whole ? __ldg(reinterpret_cast<const uint32_t *>(p) + i) : 0u;
+      }
+#pragma unroll
+      for (int u = 0; u < REALIGN_AHEAD; ++u) {
+        const int64_t q = q0 + 32 * u;
+        const uint8_t *p = from + q * 16;
+        if (q >= pieces) break;
+        if (p - shift >= m.from && p - shift + 20 <= end) {
+          const uint32_t bits = (uint32_t)shift * 8;
+          to[q] = make_uint4(__funnelshift_r(w[u][0], w[u][1], bits), __funnelshift_r(w[u][1], w[u][2], bits),
+                             __funnelshift_r(w[u][2], w[u][3], bits), __funnelshift_r(w[u][3], w[u][4], bits));
+        } else {
+          for (int i = 0; i < 16 && q * 16 + i < m.bytes; ++i) reinterpret_cast<uint8_t *>(to + q)[i] = __ldg(p + i);
+        }
+      }
+    }
+  }
+}
+
+// Rows of the groups as zeros, for an inner axis without elements.
+__global__ void __launch_bounds__(256) zero_rows_kernel(uint16_t *out, const int32_t *offsets, int groups, int rows, int64_t cols) {
+  after_previous_kernel();
+  for (int g = 0; g < groups; ++g) {
+    const RowSpan span = group_rows(offsets, g, rows);
+    for (int64_t i = span.begin * cols + blockIdx.x * 256 + threadIdx.x; i < span.end * cols; i += (int64_t)gridDim.x * 256) out[i] = 0;
+  }
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Both operands as TMA can copy them: in place, or in memory of the stream-ordered pool that `release` gives back.
+struct Operands {
+  const void *a, *b;
+  int64_t a_pitch, b_pitch;  // elements
+  void *memory = nullptr;
+
+  // a: a_rows x a_cols; b: stack matrices of b_rows x b_cols, of which a call uses those of groups with rows (stack 0: one, all of it)
+  cudaError_t align(const void *a_, int64_t a_rows, int64_t a_cols, const void *b_, int64_t stack, int64_t b_rows, int64_t b_cols,
+                    int64_t size, const int32_t *offsets, int64_t rows, const DeviceInfo &dev, cudaMemPool_t pool, cudaStream_t s,
+                    int64_t *launches) {
+    a = a_;
+    b = b_;
+    a_pitch = a_cols;
+    b_pitch = b_cols;
+    const bool move_a = !aligned16(a) || a_cols * size % 16 != 0, move_b = !aligned16(b) || b_cols * size % 16 != 0;
+    if (!move_a && !move_b) return cudaSuccess;
+    auto padded = [&](int64_t cols) { return (cols * size + 15) / 16 * 16; };
+    const int64_t b_all = (stack > 0 ? stack : 1) * b_rows;
+    const int64_t a_bytes = move_a ? a_rows * padded(a_cols) : 0, b_bytes = move_b ? b_all * padded(b_cols) : 0;
+    cudaError_t e = cudaMallocFromPoolAsync(&memory, (size_t)(a_bytes + b_bytes), pool, s);
+    if (e != cudaSuccess) return e;
+    Realigned ra = {}, rb = {};
+    if (move_a) {
+      ra = {static_cast<const uint8_t *>(a_), static_cast<uint8_t *>(memory), a_rows, a_cols * size, padded(a_cols), 0};
+      a = ra.to;
+      a_pitch = ra.pitch / size;
+    }
+    if (move_b) {
+      rb = {static_cast<const uint8_t *>(b_), static_cast<uint8_t *>(memory) + a_bytes, b_all, b_cols * size, padded(b_cols),
+            stack > 0 && offsets ? b_rows : 0};
+      b = rb.to;
+      b_pitch = rb.pitch / size;
+    }
+    ++*launches;
+    const int64_t blocks = ceil_div(ra.rows + rb.rows, REALIGN_THREADS / 32), most = 8 * (int64_t)dev.sm_count;
+    e = launch_chained(realign_kernel, (unsigned)(blocks < most ? blocks : most), REALIGN_THREADS, 0, s, ra, rb, offsets, (int)rows);
+    return e != cudaSuccess ? e : cudaGetLastError();
+  }
+  cudaError_t release(cudaStream_t s, cudaError_t e) {
+    const cudaError_t freed = memory ? cudaFreeAsync(memory, s) : cudaSuccess;
+    return e != cudaSuccess ? e : freed;
+  }
+};
 
 // Opts a kernel into its shared memory, once per device; racing threads repeat an idempotent call.
 template <class S>
@@ -940,8 +1061,6 @@ cudaError_t launch(const CUtensorMap &map_l, const CUtensorMap &map_t, const Pro
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 // kind::f16 and kind::f8f6f4: f32 sums (bits 4-5), types of A and B (bits 7-9, 10-12), MN-major A and B (bits 15, 16),
 // N >> 3 (bits 17-22, per tile), M >> 4 (bits 24-28).
 uint32_t instruction_descriptor(int a_type, int b_type, bool a_mn, bool b_mn, int m) {
@@ -951,14 +1070,14 @@ uint32_t instruction_descriptor(int a_type, int b_type, bool a_mn, bool b_mn, in
 }
 
 template <int CTAS, int TILE, bool FP8, bool MN>
-cudaError_t launch_rows(const GroupedArgs &a, Product p, int parts, const DeviceInfo &dev, cudaStream_t s) {
+cudaError_t launch_rows(const GroupedArgs &a, const Operands &from, Product p, int parts, const DeviceInfo &dev, cudaStream_t s) {
   using S = Config<CTAS, TILE, FP8, MN, false>;
   CUtensorMap map_l, map_t;
   const int b_type = FP8 ? a.b_type : a.type;
   // (rows on the lanes: boxes of 128 rows or columns of either operand)
-  const bool made = (MN ? make_map(&map_l, a.B, b_type, a.n, a.inner, a.groups, S::STEP)
-                        : make_map(&map_l, a.B, b_type, a.inner, a.n, a.groups, LANES)) &&
-                    make_map(&map_t, a.A, a.type, a.inner, a.rows, 0, S::ROW_BOX);
+  const bool made = (MN ? make_map(&map_l, from.b, b_type, a.n, a.inner, a.groups, from.b_pitch, S::STEP)
+                        : make_map(&map_l, from.b, b_type, a.inner, a.n, a.groups, from.b_pitch, LANES)) &&
+                    make_map(&map_t, from.a, a.type, a.inner, a.rows, 0, from.a_pitch, S::ROW_BOX);
   if (!made) return cudaErrorInvalidValue;
   p.instruction = S::ROWS_ON_LANES ? instruction_descriptor(a.type, b_type, false, MN, LANES * CTAS)
                                    : instruction_descriptor(b_type, a.type, MN, false, LANES * CTAS);
@@ -971,13 +1090,20 @@ constexpr int64_t NARROW_ROWS = 64;
 
 }  // namespace
 
-bool grouped_rows_tcgen05_supported(const GroupedArgs &a) {
-  const int64_t size = a.a_scales ? 1 : 2, pitch = a.transpose_b ? a.inner : a.n;
-  return a.inner > 0 && a.rows > 0 && a.inner * size % 16 == 0 && pitch * size % 16 == 0 && aligned16(a.A) && aligned16(a.B);
-}
-
-cudaError_t launch_grouped_rows_tcgen05(const GroupedArgs &a, int *status_flag, const DeviceInfo &dev, cudaStream_t s,
-                                        int64_t *launches) {
+cudaError_t launch_grouped_rows_tcgen05(const GroupedArgs &a, int *status_flag, const DeviceInfo &dev, cudaMemPool_t pool,
+                                        cudaStream_t s, int64_t *launches) {
+  if (a.rows == 0) return cudaSuccess;
+  if (a.inner == 0) {
+    ++*launches;
+    const cudaError_t e = launch_chained(zero_rows_kernel, (unsigned)dev.sm_count, 256, 0, s, static_cast<uint16_t *>(a.C), a.offsets,
+                                         (int)a.groups, (int)a.rows, a.n);
+    return e != cudaSuccess ? e : cudaGetLastError();
+  }
+  const bool fp8 = a.a_scales != nullptr;
+  Operands from;
+  cudaError_t e = from.align(a.A, a.rows, a.inner, a.B, a.groups, a.transpose_b ? a.n : a.inner, a.transpose_b ? a.inner : a.n,
+                             fp8 ? 1 : 2, a.offsets, a.rows, dev, pool, s, launches);
+  if (e != cudaSuccess) return from.release(s, e);
   ++*launches;
   Product p = {};
   p.rows = (int)a.rows;
@@ -986,39 +1112,40 @@ cudaError_t launch_grouped_rows_tcgen05(const GroupedArgs &a, int *status_flag, 
   p.groups = (int)a.groups;
   p.offsets = a.offsets;
   p.out = static_cast<uint16_t *>(a.C);
-  p.half_out = !a.a_scales && a.type == kF16;
+  p.half_out = !fp8 && a.type == kF16;
   p.a_scales = a.a_scales;
   p.b_scales = a.b_scales;
   const int64_t kb = ceil_div(a.inner, kScaleBlock), nb = ceil_div(a.n, kScaleBlock);
   p.scale_k = (int)(a.transpose_b ? 1 : nb);
   p.scale_j = (int)(a.transpose_b ? kb : 1);
-  p.scale_group = (int)(kb * nb);
+  p.scale_group = kb * nb;
   p.status = status_flag;
   const int64_t active = a.groups < a.rows ? a.groups : a.rows;
-  if (a.rows <= NARROW_ROWS * active) {
-    const int64_t tiles = active * ceil_div(a.n, LANES), steps = ceil_div(a.inner, a.a_scales ? 128 : 64);
-    int parts = 1;
+  const bool narrow = a.rows <= NARROW_ROWS * active, mn = !a.transpose_b;
+  int parts = 1;
+  if (narrow) {
+    const int64_t tiles = active * ceil_div(a.n, LANES), steps = ceil_div(a.inner, fp8 ? 128 : 64);
     while (parts < 8 && tiles * parts * 2 <= dev.sm_count && steps >= parts * 4) parts *= 2;
-    if (a.a_scales)
-      return a.transpose_b ? launch_rows<1, 64, true, false>(a, p, parts, dev, s) : launch_rows<1, 64, true, true>(a, p, parts, dev, s);
-    return a.transpose_b ? launch_rows<1, 64, false, false>(a, p, parts, dev, s) : launch_rows<1, 64, false, true>(a, p, parts, dev, s);
   }
-  if (a.a_scales)
-    return a.transpose_b ? launch_rows<2, 256, true, false>(a, p, 1, dev, s) : launch_rows<2, 256, true, true>(a, p, 1, dev, s);
-  return a.transpose_b ? launch_rows<2, 256, false, false>(a, p, 1, dev, s) : launch_rows<2, 256, false, true>(a, p, 1, dev, s);
+  if (narrow && fp8) e = mn ? launch_rows<1, 64, true, true>(a, from, p, parts, dev, s) : launch_rows<1, 64, true, false>(a, from, p, parts, dev, s);
+  else if (narrow) e = mn ? launch_rows<1, 64, false, true>(a, from, p, parts, dev, s) : launch_rows<1, 64, false, false>(a, from, p, parts, dev, s);
+  else if (fp8) e = mn ? launch_rows<2, 256, true, true>(a, from, p, 1, dev, s) : launch_rows<2, 256, true, false>(a, from, p, 1, dev, s);
+  else e = mn ? launch_rows<2, 256, false, true>(a, from, p, 1, dev, s) : launch_rows<2, 256, false, false>(a, from, p, 1, dev, s);
+  return from.release(s, e);
 }
 
-bool grouped_inner_tcgen05_supported(const GroupedInnerArgs &a) {
-  return a.rows > 0 && a.i_size % 8 == 0 && a.j_size % 8 == 0 && aligned16(a.left) && aligned16(a.right);
-}
-
-cudaError_t launch_grouped_inner_tcgen05(const GroupedInnerArgs &a, int *status_flag, const DeviceInfo &dev, cudaStream_t s,
-                                         int64_t *launches) {
+cudaError_t launch_grouped_inner_tcgen05(const GroupedInnerArgs &a, int *status_flag, const DeviceInfo &dev, cudaMemPool_t pool,
+                                         cudaStream_t s, int64_t *launches) {
+  if (a.rows == 0) return cudaMemsetAsync(a.out, 0, (size_t)(a.groups * a.i_size * a.j_size) * 2, s);
+  Operands from;
+  cudaError_t e = from.align(a.left, a.rows, a.i_size, a.right, 0, a.rows, a.j_size, 2, nullptr, a.rows, dev, pool, s, launches);
+  if (e != cudaSuccess) return from.release(s, e);
   ++*launches;
   using S = Config<2, 256, false, true, true>;
   CUtensorMap map_l, map_t;
-  if (!make_map(&map_l, a.right, a.type, a.j_size, a.rows, 0, S::STEP) || !make_map(&map_t, a.left, a.type, a.i_size, a.rows, 0, S::ROW_BOX))
-    return cudaErrorInvalidValue;
+  if (!make_map(&map_l, from.b, a.type, a.j_size, a.rows, 0, from.b_pitch, S::STEP) ||
+      !make_map(&map_t, from.a, a.type, a.i_size, a.rows, 0, from.a_pitch, S::ROW_BOX))
+    return from.release(s, cudaErrorInvalidValue);
   Product p = {};
   p.rows = (int)a.rows;
   p.inner = (int)a.i_size;
@@ -1030,7 +1157,7 @@ cudaError_t launch_grouped_inner_tcgen05(const GroupedInnerArgs &a, int *status_
   p.status = status_flag;
   p.instruction = instruction_descriptor(a.type, a.type, true, true, LANES * 2);
   const int64_t tiles = a.groups * ceil_div(a.i_size, S::TILE) * ceil_div(a.j_size, LANES * 2);
-  return launch<S>(map_l, map_t, p, tiles, 1, dev.sm_count, s);
+  return from.release(s, launch<S>(map_l, map_t, p, tiles, 1, dev.sm_count, s));
 }
 
 }  // namespace swb

@@ -36,6 +36,8 @@ struct swb_context {
   void *band_scratch = nullptr;
   size_t band_scratch_bytes = 0;
   int *status_flag = nullptr;  // device int for kernels with bounded waits
+  // Stream-ordered memory of calls that copy an operand first (a call's own, in a captured graph the graph's); kept by the pool.
+  cudaMemPool_t pool = nullptr;
   // Sharded operators: device copy of this rank's chunk of the dense operand padded to the common chunk
   // size, and the gathered operand when no peer window serves (both grown on demand, kept).
   char *shard_send = nullptr, *shard_full = nullptr;
@@ -87,6 +89,7 @@ void set_context_peer_window(swb_context *ctx, void *window) { ctx->peer_window 
 int *context_status_flag(const swb_context *ctx) { return ctx->status_flag; }
 const DeviceInfo &context_device_info(const swb_context *ctx) { return ctx->dev; }
 int64_t *context_launches(swb_context *ctx) { return &ctx->launches; }
+cudaMemPool_t context_pool(const swb_context *ctx) { return ctx->pool; }
 void count_launch(swb_context *ctx) { ++ctx->launches; }
 }  // namespace swb
 
@@ -240,7 +243,18 @@ int swb_create(swb_context **out_ctx, int device_ordinal) {
   // Status word of kernels with bounded waits (0 = no wait ever gave up).
   e = cudaMalloc(&ctx->status_flag, sizeof(int));
   if (e == cudaSuccess) e = cudaMemset(ctx->status_flag, 0, sizeof(int));
+  if (e == cudaSuccess) {
+    cudaMemPoolProps props = {};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = device_ordinal;
+    e = cudaMemPoolCreate(&ctx->pool, &props);
+    uint64_t keep = UINT64_MAX;
+    if (e == cudaSuccess) e = cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &keep);
+  }
   if (e != cudaSuccess) {
+    if (ctx->status_flag) cudaFree(ctx->status_flag);
+    if (ctx->pool) cudaMemPoolDestroy(ctx->pool);
     delete ctx;
     return cuda_fail(nullptr, e, "cudaMalloc(status)");
   }
@@ -270,6 +284,7 @@ void swb_destroy(swb_context *ctx) {
   if (ctx->shard_send) cudaFree(ctx->shard_send);
   if (ctx->shard_full) cudaFree(ctx->shard_full);
   if (ctx->status_flag) cudaFree(ctx->status_flag);
+  if (ctx->pool) cudaMemPoolDestroy(ctx->pool);
   if (ctx->host_stream) cudaStreamDestroy(ctx->host_stream);
   if (ctx->copy_stream) cudaStreamDestroy(ctx->copy_stream);
   if (ctx->upload_stream) cudaStreamDestroy(ctx->upload_stream);

@@ -46,18 +46,12 @@ int check_grouped(swb_context *ctx, const char *op, int64_t rows, int64_t inner,
 }
 
 cudaError_t rows_product(swb_context *ctx, const swb::GroupedArgs &a, swb_stream stream) {
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int64_t *launches = swb::context_launches(ctx);
-  return swb::grouped_rows_tcgen05_supported(a)
-             ? swb::launch_grouped_rows_tcgen05(a, swb::context_status_flag(ctx), swb::context_device_info(ctx), s, launches)
-             : swb::launch_grouped_rows_general(a, s, launches);
+  return swb::launch_grouped_rows_tcgen05(a, swb::context_status_flag(ctx), swb::context_device_info(ctx), swb::context_pool(ctx),
+                                          static_cast<cudaStream_t>(stream), swb::context_launches(ctx));
 }
 cudaError_t inner_product(swb_context *ctx, const swb::GroupedInnerArgs &a, swb_stream stream) {
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int64_t *launches = swb::context_launches(ctx);
-  return swb::grouped_inner_tcgen05_supported(a)
-             ? swb::launch_grouped_inner_tcgen05(a, swb::context_status_flag(ctx), swb::context_device_info(ctx), s, launches)
-             : swb::launch_grouped_inner_general(a, s, launches);
+  return swb::launch_grouped_inner_tcgen05(a, swb::context_status_flag(ctx), swb::context_device_info(ctx), swb::context_pool(ctx),
+                                           static_cast<cudaStream_t>(stream), swb::context_launches(ctx));
 }
 
 bool is_fp8(int32_t type) { return type == SWB_E4M3 || type == SWB_E5M2; }

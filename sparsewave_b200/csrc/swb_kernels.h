@@ -179,15 +179,11 @@ cudaError_t launch_bsr_spmm_tcgen05(const BsrSpmmArgs &a, int *status_flag, cons
                                     int64_t *launches);
 
 // --- products grouped by expert, 8-bit operands
-cudaError_t launch_grouped_rows_general(const GroupedArgs &a, cudaStream_t s, int64_t *launches);
-cudaError_t launch_grouped_inner_general(const GroupedInnerArgs &a, cudaStream_t s, int64_t *launches);
-// The same on the tcgen05 tensor cores: operands and their rows on 16-byte boundaries, an inner axis.  `status_flag` as for BSR.
-bool grouped_rows_tcgen05_supported(const GroupedArgs &a);
-cudaError_t launch_grouped_rows_tcgen05(const GroupedArgs &a, int *status_flag, const DeviceInfo &dev, cudaStream_t s,
-                                        int64_t *launches);
-bool grouped_inner_tcgen05_supported(const GroupedInnerArgs &a);
-cudaError_t launch_grouped_inner_tcgen05(const GroupedInnerArgs &a, int *status_flag, const DeviceInfo &dev, cudaStream_t s,
-                                         int64_t *launches);
+// On the tcgen05 tensor cores.  `status_flag` as for BSR; `pool` gives memory for copies of operands that TMA cannot read in place.
+cudaError_t launch_grouped_rows_tcgen05(const GroupedArgs &a, int *status_flag, const DeviceInfo &dev, cudaMemPool_t pool,
+                                        cudaStream_t s, int64_t *launches);
+cudaError_t launch_grouped_inner_tcgen05(const GroupedInnerArgs &a, int *status_flag, const DeviceInfo &dev, cudaMemPool_t pool,
+                                         cudaStream_t s, int64_t *launches);
 cudaError_t launch_quantize_rows(const QuantizeArgs &a, cudaStream_t s, int64_t *launches);
 cudaError_t launch_quantize_blocks(const QuantizeArgs &a, cudaStream_t s, int64_t *launches);
 
@@ -210,6 +206,7 @@ void abandon_peer_window(swb_context *ctx);  // non-collective tear-down (swb_pe
 int *context_status_flag(const swb_context *ctx);
 const DeviceInfo &context_device_info(const swb_context *ctx);
 int64_t *context_launches(swb_context *ctx);
+cudaMemPool_t context_pool(const swb_context *ctx);
 void count_launch(swb_context *ctx);
 
 // Stores the diagnostic that swb_last_error(NULL) returns on this thread.
