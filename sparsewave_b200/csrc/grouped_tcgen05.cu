@@ -20,7 +20,7 @@
 // rows themselves and shift them into place for every tile took 62 us, the copy and the product 24.)
 //
 // Roles: warp 0 copies, warp 1 issues the MMAs, warp 2 clears the rows behind a group's last (inner form),
-// four warps (wide 8-bit: eight) from warp 4 on read the accumulators, round and store.
+// four warps (wide tiles: eight) from warp 4 on read the accumulators, round and store.
 //
 // The inner form has rows of the result on the lanes, whose results then lie in a row in each lane's registers.  Wide 8-bit tiles
 // have their rows on the lanes too, and 256 columns of the weights as accumulator columns: a row's scale is then one
@@ -64,18 +64,33 @@ struct Config {
   static constexpr int L_BYTES = LANES * ROW_BYTES, T_BYTES = ROWS_CTA * ROW_BYTES, STAGE = L_BYTES + T_BYTES;
   static constexpr int BUFFERS = 512 / TILE < 4 ? 512 / TILE : 4;
   static constexpr int TMEM_COLS = BUFFERS * TILE;
-  static constexpr int STORE_WARPS = FP8 && TILE == 256 ? 8 : 4;
+  static constexpr int STORE_WARPS = CTAS == 2 ? 8 : 4;
   static constexpr int WARP_COLS = TILE / (STORE_WARPS / 4);  // accumulator columns of a storing warp
   static constexpr int THREADS = 32 * (FIRST_STORE_WARP + STORE_WARPS);
   static constexpr bool SPLITS = CTAS == 1 && !INNER;
   static constexpr int PARTIAL = SPLITS ? TILE * LANES * 4 : 0;       // f32 sums of this CTA's share of the inner axis
   static constexpr int SCALES = FP8 && !ROWS_ON_LANES ? STORE_WARPS * 4 * WARP_COLS * 4 : 0;
-  static constexpr int OUT_PITCH = 80;                                // 32 x 32 results of a warp on their way to rows of C
-  static constexpr int STAGED = STORE_WARPS * 32 * OUT_PITCH;
-  static constexpr int TABLE = (int)kMaxGroups * 12 + 16;             // spans and tile counts
+  static constexpr int STAGED = STORE_WARPS * 32 * 64;                // 32 x 32 results of a warp on their way to rows of C
+  static constexpr int TABLE = (int)kMaxGroups * 16 + 16;             // GroupTiles, and first tiles
   static constexpr int STAGES = (232448 - 1024 - 512 - PARTIAL - SCALES - STAGED - TABLE) / STAGE;
   static constexpr int SMEM = 1024 + STAGES * STAGE + PARTIAL + SCALES + STAGED + TABLE;
   static constexpr int ROUND = 16 * CTAS;                             // N of an MMA is a multiple of this
+};
+
+// Division by a number known beforehand: the product with 2^32 / d, rounded down, gives the quotient or one less.
+struct Divisor {
+  uint32_t d, inverse;
+
+  __host__ __device__ static Divisor of(uint32_t d) { return {d, d > 1 ? (uint32_t)((1ull << 32) / d) : 0xffffffffu}; }
+  __device__ __forceinline__ int divide(int x, int *rest) const {
+    uint32_t q = __umulhi((uint32_t)x, inverse), r = (uint32_t)x - q * d;
+    if (r >= d) {
+      ++q;
+      r -= d;
+    }
+    *rest = (int)r;
+    return (int)q;
+  }
 };
 
 struct Product {
@@ -85,6 +100,9 @@ struct Product {
   uint32_t instruction;           // descriptor without N
   bool half_out;
   const float *a_scales, *b_scales;
+  int col_tiles;                  // tiles along the columns
+  Divisor per_band;               // tiles of eight row tiles
+  Divisor per_group, per_column;  // inner form: tiles of a group, of a column of tiles
   int scale_k, scale_j;
   int64_t scale_group;
   int *status;
@@ -239,11 +257,26 @@ __device__ __forceinline__ uint32_t rounded_two(float lo, float hi, bool half_ou
   return r;
 }
 
-// Row tiles of a group of m rows: as few as the tile size allows, of equal heights but for the last.
-__device__ __forceinline__ void row_tiles(int m, int tile, int round, int *count, int *height) {
-  *count = (m + tile - 1) / tile;
-  *height = *count ? ((m + *count - 1) / *count + round - 1) / round * round : round;
+__device__ __forceinline__ Divisor up_to_eight(int d) {
+  const uint32_t inverse = d == 1 ? 0xffffffffu : d == 2 ? 1u << 31 : d == 3 ? 0x55555555u : d == 4 ? 1u << 30 : d == 5 ? 0x33333333u
+                           : d == 6 ? 0x2aaaaaaau : d == 7 ? 0x24924924u : 1u << 29;
+  return {(uint32_t)d, inverse};
 }
+
+// A group's rows, and its row tiles: as few as the tile size allows, of equal heights (a multiple of 16) but for the last.
+struct GroupTiles {
+  int begin, end;
+  uint32_t packed;
+
+  template <class S>
+  __device__ __forceinline__ static GroupTiles of(RowSpan span) {
+    const int m = span.end - span.begin, count = (m + S::TILE - 1) / S::TILE;
+    const int height = count ? ((m + count - 1) / count + S::ROUND - 1) / S::ROUND * S::ROUND : S::ROUND;
+    return {span.begin, span.end, (uint32_t)count << 5 | (uint32_t)(height / 16)};
+  }
+  __device__ __forceinline__ int count() const { return (int)(packed >> 5); }
+  __device__ __forceinline__ int height() const { return (int)(packed & 31u) * 16; }
+};
 
 struct Tile {
   int group, row0, valid;     // rows [row0, row0 + valid) (inner form: of axis i)
@@ -267,24 +300,24 @@ __device__ __forceinline__ Tile uniform(const Tile &t) {  // the same in all lan
 
 template <class S>
 struct Tiles {
-  const int2 *spans;
+  const GroupTiles *spans;
   const int *first;  // first tile of each group, and the end
-  int groups, total, col_tiles, inner_tiles;
+  int groups, total;
 
   __device__ __forceinline__ Tile at(int t, const Product &p, int part, int parts) const {
     Tile tile;
     if constexpr (S::INNER) {
-      const int per_group = col_tiles * inner_tiles;
-      tile.group = t / per_group;
-      const int local = t - tile.group * per_group, it = local % inner_tiles;
-      tile.col0 = local / inner_tiles * (LANES * S::CTAS);
+      static_assert(S::TILE == LANES * S::CTAS, "");  // square tiles
+      int local, it;
+      tile.group = p.per_group.divide(t, &local);
+      tile.col0 = p.per_column.divide(local, &it) * (LANES * S::CTAS);
       tile.row0 = it * S::TILE;
       tile.valid = p.inner - tile.row0 < S::TILE ? p.inner - tile.row0 : S::TILE;
       const int n = p.cols - tile.col0 < S::TILE ? p.cols - tile.col0 : S::TILE;
       tile.n = (n + S::ROUND - 1) / S::ROUND * S::ROUND;
-      const int2 span = spans[tile.group];
-      const int m = span.y - span.x;
-      tile.k0 = span.x;
+      const GroupTiles span = spans[tile.group];
+      const int m = span.end - span.begin;
+      tile.k0 = span.begin;
       tile.k_blocks = (m + S::STEP - 1) / S::STEP;
       tile.k_valid = m - (tile.k_blocks - 1) * S::STEP;
     } else {
@@ -294,16 +327,14 @@ struct Tiles {
         if (first[mid] <= t) lo = mid; else hi = mid;
       }
       tile.group = lo;
-      const int2 span = spans[lo];
-      int count, height;
-      row_tiles(span.y - span.x, S::TILE, S::ROUND, &count, &height);
+      const GroupTiles span = spans[lo];
       // bands of eight row tiles, column tile after column tile within one: what runs at a time shares both operands in L2
-      const int local = t - first[lo], band = local / (8 * col_tiles), in_band = local - band * 8 * col_tiles;
-      const int band_rows = count - band * 8 < 8 ? count - band * 8 : 8;
-      const int row_tile = band * 8 + in_band % band_rows;
-      tile.col0 = in_band / band_rows * (LANES * S::CTAS);
-      tile.row0 = span.x + row_tile * height;
-      tile.valid = span.y - tile.row0 < height ? span.y - tile.row0 : height;
+      int in_band, in_rows;
+      const int band = p.per_band.divide(t - first[lo], &in_band);
+      const int left = span.count() - band * 8;
+      tile.col0 = up_to_eight(left < 8 ? left : 8).divide(in_band, &in_rows) * (LANES * S::CTAS);
+      tile.row0 = span.begin + (band * 8 + in_rows) * span.height();
+      tile.valid = span.end - tile.row0 < span.height() ? span.end - tile.row0 : span.height();
       int n = tile.valid;
       if constexpr (S::ROWS_ON_LANES) n = p.cols - tile.col0 < S::TILE ? p.cols - tile.col0 : S::TILE;
       tile.n = (n + S::ROUND - 1) / S::ROUND * S::ROUND;
@@ -332,7 +363,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   float *partial = reinterpret_cast<float *>(behind);                         // [TILE][LANES]
   float *scales = reinterpret_cast<float *>(behind + S::PARTIAL);             // [warp][4][WARP_COLS]
   uint8_t *staged_all = behind + S::PARTIAL + S::SCALES;
-  int2 *spans = reinterpret_cast<int2 *>(staged_all + S::STAGED);
+  GroupTiles *spans = reinterpret_cast<GroupTiles *>(staged_all + S::STAGED);
   int *first = reinterpret_cast<int *>(spans + kMaxGroups);
   const int rank = S::CTAS == 2 || S::SPLITS ? (int)(blockIdx.x % (unsigned)(S::CTAS == 2 ? 2 : parts)) : 0;
   const int part = S::CTAS == 2 ? 0 : rank;  // of the inner axis
@@ -371,20 +402,13 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   tiles.spans = spans;
   tiles.first = first;
   tiles.groups = p.groups;
-  tiles.col_tiles = (p.cols + LANES * S::CTAS - 1) / (LANES * S::CTAS);
-  tiles.inner_tiles = (p.inner + S::TILE - 1) / S::TILE;
-  for (int g = tid; g < p.groups; g += S::THREADS) {
-    const RowSpan span = group_rows(p.offsets, g, p.rows);
-    spans[g] = make_int2(span.begin, span.end);
-  }
+  for (int g = tid; g < p.groups; g += S::THREADS) spans[g] = GroupTiles::of<S>(group_rows(p.offsets, g, p.rows));
   __syncthreads();
   if constexpr (!S::INNER) {
     if (warp == 0) {
       int before = 0;
       for (int g0 = 0; g0 < p.groups; g0 += 32) {
-        int count = 0, height;
-        if (g0 + lane < p.groups) row_tiles(spans[g0 + lane].y - spans[g0 + lane].x, S::TILE, S::ROUND, &count, &height);
-        int through = count * tiles.col_tiles;
+        int through = g0 + lane < p.groups ? spans[g0 + lane].count() * p.col_tiles : 0;
         const int own = through;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -405,7 +429,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = __shfl_sync(FULL, tmem_slot, 0);
-  tiles.total = S::INNER ? p.groups * tiles.col_tiles * tiles.inner_tiles : __shfl_sync(FULL, first[p.groups], 0);
+  tiles.total = S::INNER ? p.groups * (int)p.per_group.d : __shfl_sync(FULL, first[p.groups], 0);
 
   auto gave_up = [&] {
     failed = 1;
@@ -417,7 +441,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   // The eight storing warps of the wide 8-bit form need more registers than 12 warps can have alike: 128 x 56 + 256 x 224 are the
   // 384 x 168 of the launch.
   if (warp < FIRST_STORE_WARP) {
-    if constexpr (S::STORE_WARPS == 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if constexpr (S::FP8 && S::CTAS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0) {
       int s = 0;
       uint32_t round = 0;
@@ -562,7 +586,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
       }
     }
   } else {
-    if constexpr (S::STORE_WARPS == 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    if constexpr (S::FP8 && S::CTAS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int store_warp = warp - FIRST_STORE_WARP, quarter = warp & 3;
     const int c0 = store_warp / 4 * S::WARP_COLS;  // first accumulator column of this warp
     const uint32_t lanes_at = (uint32_t)(quarter * 32) << 16;
@@ -585,13 +609,15 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
       ++made;
     };
     // 32 x 32 results of the warp go to rows of C by way of shared memory: four lanes store 64 adjacent bytes of a row.
-    uint8_t *staged = staged_all + store_warp * 32 * S::OUT_PITCH;
+    // Rows of 64 bytes, whose four pieces of 16 change places from row pair to row pair: eight rows' pieces lie in different banks.
+    uint8_t *staged = staged_all + store_warp * 32 * 64;
+    auto place = [](int row, int piece) { return row * 64 + ((piece ^ (row >> 1 & 3)) * 16); };
     const bool vectors = p.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
     auto lay_down = [&](const uint32_t (&w)[16]) {  // the lane's row
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<uint4 *>(staged + lane * S::OUT_PITCH + i * 16) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        *reinterpret_cast<uint4 *>(staged + place(lane, i)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     };
     auto store_block = [&](uint16_t *out, int row0, int rows_end, int col0) {
       __syncwarp();
@@ -599,14 +625,14 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = i * 8 + lane / 4, piece = lane % 4;
-          const uint4 v = *reinterpret_cast<const uint4 *>(staged + r * S::OUT_PITCH + piece * 16);
+          const uint4 v = *reinterpret_cast<const uint4 *>(staged + place(r, piece));
           if (row0 + r < rows_end && col0 + piece * 8 < p.cols)
             *reinterpret_cast<uint4 *>(out + (int64_t)(row0 + r) * p.cols + col0 + piece * 8) = v;
         }
       } else if (col0 + lane < p.cols) {
         const int count = rows_end - row0 < 32 ? rows_end - row0 : 32;
         for (int r = 0; r < count; ++r)
-          out[(int64_t)(row0 + r) * p.cols + col0 + lane] = *reinterpret_cast<const uint16_t *>(staged + r * S::OUT_PITCH + lane * 2);
+          out[(int64_t)(row0 + r) * p.cols + col0 + lane] = *reinterpret_cast<const uint16_t *>(staged + place(r, lane / 8) + lane % 8 * 2);
       }
     };
     for (int t = walker; ok && t < tiles.total; t += walkers) {
@@ -616,12 +642,14 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
         const bool empty = tile.k_blocks == 0;  // a group without rows: zeros
         if (!empty && !wait_sums(buffer)) break;
         uint16_t *out = p.out + (int64_t)tile.group * p.inner * p.cols;
-        for (int c = 0; c < tile.n; c += 32) {
+        const int c_end = tile.n < c0 + S::WARP_COLS ? tile.n : c0 + S::WARP_COLS;
+        if (!empty && c0 >= tile.n) release_sums(buffer);
+        for (int c = c0; c < c_end; c += 32) {
           uint32_t v[32], w[16];
           if (!empty) {
             tmem_load(v, tmem + lanes_at + (uint32_t)(buffer * S::TILE + c));
             tmem_wait_loads();
-            if (c + 32 >= tile.n) release_sums(buffer);
+            if (c + 32 >= c_end) release_sums(buffer);
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -710,13 +738,15 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
             break;
           }
         }
-        for (int c = 0; c < tile.valid; c += 32) {
+        const int c_end = tile.valid < c0 + S::WARP_COLS ? tile.valid : c0 + S::WARP_COLS;
+        if (c0 >= tile.valid) release_sums(buffer);
+        for (int c = c0; c < c_end; c += 32) {
           const uint32_t at = tmem + lanes_at + (uint32_t)(buffer * S::TILE + c);
           if (split) {
             uint32_t v[32];
             tmem_load(v, at);
             tmem_wait_loads();
-            if (c + 32 >= tile.valid) release_sums(buffer);
+            if (c + 32 >= c_end) release_sums(buffer);
 #pragma unroll
             for (int i = 0; i < 32; ++i) partial[(c + i) * LANES + quarter * 32 + lane] = __uint_as_float(v[i]);
             continue;
@@ -727,7 +757,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
           tmem_load_blocks(v[0], at);
           tmem_load_blocks(v[1], at + (16u << 16));
           tmem_wait_loads();
-          if (c + 32 >= tile.valid) release_sums(buffer);
+          if (c + 32 >= c_end) release_sums(buffer);
           __syncwarp();
 #pragma unroll
           for (int h = 0; h < 2; ++h)
@@ -740,7 +770,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
                 w[m] = rounded_two(__uint_as_float(v[h][r]), __uint_as_float(v[h][r + 1]), p.half_out);
               }
               const int m = lane / 8;
-              const uint32_t to = smem_u32(staged) + (uint32_t)((8 * (i + m / 2) + lane % 8) * S::OUT_PITCH + (h * 16 + m % 2 * 8) * 2);
+              const uint32_t to = smem_u32(staged) + (uint32_t)place(8 * (i + m / 2) + lane % 8, h * 2 + m % 2);
               asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]),
                            "r"(w[2]), "r"(w[3]) : "memory");
             }
@@ -814,6 +844,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
           for (int i = 0; i < S::WARP_COLS; i += 2) {
             uint32_t lo, hi;
             unpack(sum[i / 2], lo, hi);
+            if (c0 + i >= tile.valid) break;
             partial[(c0 + i) * LANES + quarter * 32 + lane] = __uint_as_float(lo);
             partial[(c0 + i + 1) * LANES + quarter * 32 + lane] = __uint_as_float(hi);
           }
@@ -829,7 +860,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
       }
       if constexpr (S::SPLITS) {
         if (parts > 1) {
-          // Each warp's sums lie in its CTA's shared memory; the CTAs of the cluster add every `parts`-th column, in rank order.
+          // Each CTA's sums lie in its shared memory; the CTAs of the cluster add every `parts`-th row of C, in rank order.
           __syncwarp();
           if (lane < parts) mbar_arrive<true>(mapped(smem_u32(&bar_parts), (uint32_t)lane));
           ok = __all_sync(FULL, mbar_wait<true>(smem_u32(&bar_parts), shared_tiles & 1u));
@@ -837,17 +868,31 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
             if (lane == 0) gave_up();
             break;
           }
-          const uint32_t at = smem_u32(partial) + (uint32_t)(quarter * 32 + lane) * 4u;
-          for (int c = part; c < tile.valid; c += parts) {
-            float total = 0.0f, v[8];
+          // Four columns of C a lane, so that the loads of a row of C are few and on their way together.
+          const int col4 = tile.col0 + lane * 4;
+          const bool fours = p.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7u) == 0;
+          for (int c = part + parts * store_warp; c < tile.valid; c += parts * S::STORE_WARPS) {
+            const uint32_t at = smem_u32(partial) + (uint32_t)(c * LANES + lane * 4) * 4u;
+            float v[8][4], total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int r = 0; r < 8; ++r)
               if (r < parts)
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[r]) : "r"(mapped(at + (uint32_t)(c * LANES * 4), (uint32_t)r)) : "memory");
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[r][0]), "=f"(v[r][1]), "=f"(v[r][2]), "=f"(v[r][3])
+                             : "r"(mapped(at, (uint32_t)r)) : "memory");
 #pragma unroll
             for (int r = 0; r < 8; ++r)
-              if (r < parts) total += v[r];
-            if (stores) out[(int64_t)c * p.cols] = rounded(total, p.half_out);
+              if (r < parts)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) total[i] += v[r][i];
+            uint16_t *to = p.out + (int64_t)(tile.row0 + c) * p.cols + col4;
+            if (fours) {
+              if (col4 < p.cols)
+                *reinterpret_cast<uint2 *>(to) = make_uint2(rounded_two(total[0], total[1], p.half_out), rounded_two(total[2], total[3], p.half_out));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (col4 + i < p.cols) to[i] = rounded(total[i], p.half_out);
+            }
           }
           __syncwarp();
           if (lane < parts) mbar_arrive<true>(mapped(smem_u32(&bar_added), (uint32_t)lane));
@@ -1035,12 +1080,20 @@ cudaError_t configure() {
 }
 
 template <class S>
-cudaError_t launch(const CUtensorMap &map_l, const CUtensorMap &map_t, const Product &p, int64_t most_tiles, int parts, int sm_count,
+cudaError_t launch(const CUtensorMap &map_l, const CUtensorMap &map_t, Product p, int64_t most_tiles, int parts, int sm_count,
                    cudaStream_t s) {
   if (most_tiles == 0) return cudaSuccess;
   if (most_tiles > 2147483647LL - 4096) return cudaErrorInvalidConfiguration;  // tile numbers are 32-bit
   cudaError_t e = configure<S>();
   if (e != cudaSuccess) return e;
+  p.col_tiles = (int)ceil_div(p.cols, LANES * S::CTAS);
+  const int64_t inner_tiles = ceil_div(p.inner, S::TILE);
+  if (8LL * p.col_tiles > 2147483647LL || (S::INNER && p.col_tiles * inner_tiles > 2147483647LL)) return cudaErrorInvalidConfiguration;
+  p.per_band = Divisor::of(8u * (uint32_t)p.col_tiles);
+  if (S::INNER) {
+    p.per_group = Divisor::of((uint32_t)(p.col_tiles * inner_tiles));
+    p.per_column = Divisor::of((uint32_t)inner_tiles);
+  }
   const int cluster = S::CTAS == 2 ? 2 : parts;
   const int64_t walkers = most_tiles < sm_count / cluster ? most_tiles : sm_count / cluster;
   cudaLaunchAttribute attributes[2];
