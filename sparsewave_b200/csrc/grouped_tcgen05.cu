@@ -227,6 +227,13 @@ __device__ __forceinline__ void tmem_load_blocks(uint32_t (&v)[16], uint32_t add
 }
 __device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// A load that stays where it is written: the compiler moves others down to where their value is needed, to save registers.
+__device__ __forceinline__ float load_here(const float *p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+
 __device__ __forceinline__ uint64_t pack(uint32_t lo, uint32_t hi) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
@@ -665,9 +672,9 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
         uint64_t sum[S::WARP_COLS / 2];
 #pragma unroll
         for (int i = 0; i < S::WARP_COLS / 2; ++i) sum[i] = 0;
-        // The scales of four blocks at a time, asked for four blocks ahead.  Loads of places that exist, whatever the lane's row: behind
-        // a condition each would wait for the one before (eight loads some 7,000 clocks).
-        constexpr int AHEAD = 4;
+        // The scales of two blocks at a time, asked for two blocks ahead (four: 1 % slower).  Loads of places that exist, whatever the
+        // lane's row: behind a condition each would wait for the one before (eight loads some 7,000 clocks).
+        constexpr int AHEAD = 2;
         float scale[AHEAD], next_a[AHEAD], next_b[AHEAD];
         const float *a_scale = p.a_scales + (row < rows_end ? row : tile.row0);
         const float *b_scale = p.b_scales + tile.group * p.scale_group +
@@ -676,34 +683,35 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
 #pragma unroll
           for (int i = 0; i < AHEAD; ++i) {
             const int64_t block = kb + i < tile.k_blocks ? kb + i : tile.k_blocks - 1;
-            next_a[i] = __ldg(a_scale + block * p.rows);
-            next_b[i] = __ldg(b_scale + block * p.scale_k);
+            next_a[i] = load_here(a_scale + block * p.rows);
+            next_b[i] = load_here(b_scale + block * p.scale_k);
           }
         };
         fetch(0);
-        for (int k4 = 0; ok && k4 < tile.k_blocks; k4 += AHEAD) {
+        for (int k0 = 0; ok && k0 < tile.k_blocks; k0 += AHEAD) {
 #pragma unroll
           for (int i = 0; i < AHEAD; ++i) scale[i] = next_a[i] * next_b[i];
-          fetch(k4 + AHEAD);
+          fetch(k0 + AHEAD);
 #pragma unroll
           for (int k = 0; k < AHEAD; ++k) {
-            if (k4 + k >= tile.k_blocks) break;
+            if (k0 + k >= tile.k_blocks) break;
             const int buffer = (int)(made % S::BUFFERS);
             if (!wait_sums(buffer)) break;
             const uint32_t at = tmem + lanes_at + (uint32_t)(buffer * S::TILE + c0);
             const uint64_t f = pack(__float_as_uint(scale[k]), __float_as_uint(scale[k]));
-            uint32_t v[2][32];  // the loads of 32 columns run while those before are added
+            uint32_t v[2][32];  // 64 columns are loaded at a time
             if (used > 0) tmem_load(v[0], at);
+            if (used > 32) tmem_load(v[1], at + 32u);
 #pragma unroll
             for (int c = 0; c < S::WARP_COLS; c += 32) {
               uint32_t (&now)[32] = v[c / 32 % 2];
-              tmem_wait_loads();
-              if (c + 32 < S::WARP_COLS && c + 32 < used) tmem_load(v[(c / 32 + 1) % 2], at + (uint32_t)(c + 32));
-              if (c + 32 == S::WARP_COLS) release_sums(buffer);
+              if (c % 64 == 0) tmem_wait_loads();
+              if (c == 64) release_sums(buffer);
               if (c < used) {
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) sum[(c + i) / 2] = fma_two(pack(now[i], now[i + 1]), f, sum[(c + i) / 2]);
               }
+              if (c < 64 && c + 64 < used) tmem_load(now, at + (uint32_t)(c + 64));
             }
           }
         }
@@ -789,11 +797,11 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
 #pragma unroll
           for (int j = 0; j < AHEAD; ++j) {
             const int64_t block = tile.k0 + (kb + j < tile.k_blocks ? kb + j : tile.k_blocks - 1);
-            next_b[j] = __ldg(b_scale + block * p.scale_k);
+            next_b[j] = load_here(b_scale + block * p.scale_k);
 #pragma unroll
             for (int i = 0; i < PER_LANE; ++i) {
               const int c = c0 + i * 32 + lane;
-              next_a[j][i] = __ldg(p.a_scales + block * p.rows + tile.row0 + (c < tile.valid ? c : 0));
+              next_a[j][i] = load_here(p.a_scales + block * p.rows + tile.row0 + (c < tile.valid ? c : 0));
             }
           }
         };
