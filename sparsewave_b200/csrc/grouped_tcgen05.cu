@@ -8,9 +8,9 @@
 //
 // Tiles.  Wide: pairs of CTAs (cta_group::2) make 256 output columns x up to 256 rows; each CTA loads its 128 columns of the
 // weights and half of the rows, so that an operand byte feeds twice the work that it feeds in one CTA.  Narrow, for groups of few
-// rows, whose time is the reading of the weights: one CTA makes 128 columns x up to 64 rows, and a cluster of up to eight CTAs
-// shares the inner axis of a tile where there are few tiles; their sums are added through distributed shared memory, in the order
-// of the CTAs' ranks, so that results do not depend on timing and no workspace is needed.
+// rows, whose time is the reading of the weights: one CTA makes 128 columns x up to 64 (16 bits: or 128) rows, and a cluster of up
+// to eight CTAs shares the inner axis of a tile where there are few tiles; their sums are added through distributed shared memory,
+// in the order of the CTAs' ranks, so that results do not depend on timing and no workspace is needed.
 //
 // Which tile lies where is worked out on the device from the offsets: every CTA builds the table of the groups' tiles in shared
 // memory, and the CTAs (pairs, clusters) walk the tiles in turn.
@@ -1087,8 +1087,48 @@ cudaError_t configure() {
   return e;
 }
 
+// A launch of `clusters` clusters of `cluster` CTAs, set up while the kernel before it drains.
 template <class S>
-cudaError_t launch(const CUtensorMap &map_l, const CUtensorMap &map_t, Product p, int64_t most_tiles, int parts, int sm_count,
+struct LaunchShape {
+  cudaLaunchAttribute attributes[2];
+  cudaLaunchConfig_t cfg = {};
+
+  LaunchShape(int64_t clusters, int cluster, cudaStream_t s) {
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = (unsigned)cluster;
+    attributes[1].val.clusterDim.y = 1;
+    attributes[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(clusters * cluster));
+    cfg.blockDim = dim3(S::THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = s;
+    cfg.attrs = attributes;
+    cfg.numAttrs = 2;
+  }
+};
+
+// Clusters of a size that run at a time (on 148 SMs 74 of two, 33 of four, 15 of eight): asked once per device.
+template <class S>
+int resident_clusters(int cluster, const DeviceInfo &dev) {
+  static std::atomic<int> known[64][9];
+  int device = 0, n = 0;
+  cudaGetDevice(&device);
+  const bool keep = device >= 0 && device < 64 && cluster <= 8;
+  if (keep && (n = known[device][cluster].load(std::memory_order_acquire)) > 0) return n;
+  if (configure<S>() != cudaSuccess) return 1;  // the launch reports it
+  LaunchShape<S> shape(dev.sm_count, cluster, nullptr);
+  if (cudaOccupancyMaxActiveClusters(&n, grouped_tcgen05_kernel<S>, &shape.cfg) != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    return dev.sm_count / cluster > 0 ? dev.sm_count / cluster : 1;
+  }
+  if (keep) known[device][cluster].store(n, std::memory_order_release);
+  return n;
+}
+
+template <class S>
+cudaError_t launch(const CUtensorMap &map_l, const CUtensorMap &map_t, Product p, int64_t most_tiles, int parts, const DeviceInfo &dev,
                    cudaStream_t s) {
   if (most_tiles == 0) return cudaSuccess;
   if (most_tiles > 2147483647LL - 4096) return cudaErrorInvalidConfiguration;  // tile numbers are 32-bit
@@ -1103,22 +1143,9 @@ cudaError_t launch(const CUtensorMap &map_l, const CUtensorMap &map_t, Product p
     p.per_column = Divisor::of((uint32_t)inner_tiles);
   }
   const int cluster = S::CTAS == 2 ? 2 : parts;
-  const int64_t walkers = most_tiles < sm_count / cluster ? most_tiles : sm_count / cluster;
-  cudaLaunchAttribute attributes[2];
-  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attributes[0].val.programmaticStreamSerializationAllowed = 1;
-  attributes[1].id = cudaLaunchAttributeClusterDimension;
-  attributes[1].val.clusterDim.x = (unsigned)cluster;
-  attributes[1].val.clusterDim.y = 1;
-  attributes[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(walkers * cluster));
-  cfg.blockDim = dim3(S::THREADS);
-  cfg.dynamicSmemBytes = S::SMEM;
-  cfg.stream = s;
-  cfg.attrs = attributes;
-  cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, grouped_tcgen05_kernel<S>, map_l, map_t, p, parts);
+  const int64_t resident = resident_clusters<S>(cluster, dev);
+  LaunchShape<S> shape(most_tiles < resident ? most_tiles : resident, cluster, s);
+  e = cudaLaunchKernelEx(&shape.cfg, grouped_tcgen05_kernel<S>, map_l, map_t, p, parts);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
@@ -1143,11 +1170,56 @@ cudaError_t launch_rows(const GroupedArgs &a, const Operands &from, Product p, i
   p.instruction = S::ROWS_ON_LANES ? instruction_descriptor(a.type, b_type, false, MN, LANES * CTAS)
                                    : instruction_descriptor(b_type, a.type, MN, false, LANES * CTAS);
   const int64_t most = (ceil_div(a.rows, TILE) + (a.groups < a.rows ? a.groups : a.rows)) * ceil_div(a.n, LANES * CTAS);
-  return launch<S>(map_l, map_t, p, most, parts, dev.sm_count, s);
+  return launch<S>(map_l, map_t, p, most, parts, dev, s);
 }
 
-// Narrow tiles where groups have few rows.
-constexpr int64_t NARROW_ROWS = 64;
+// Which tiles, and how many CTAs share a tile's inner axis: what the host knows are the sizes, so it takes the rows to be dealt evenly
+// to as many groups as can have some, and compares times in us as measured (2048 x 1536, 1 to 64 groups of 8 to 512 rows), each
+// rounds x (stages of a CTA x time of one + what a tile costs beside them) + the launch:
+//   narrow   a stage 0.23 + 0.0006 per row (8 bits 0.45 + 0.0015), a tile 0.5, shared 1.6 + 0.024 per row, the launch 3.3;
+//   wide     a stage 0.095 + 0.00075 per row, at least 0.155 (8 bits 0.48), a tile 1.0, the launch 5.
+// us narrow (64 rows), narrow (128) and wide, measured: one group of 8 rows 6.2, -, 9.7; of 96 -, 8.3, 10.4; of 512 39, 26, 14.8;
+// 8 groups of 32 12.0, -, 10.6; of 96 20.9, 13.9, 11.9; 64 of 8 69.4, -, 69.8; of 128 100, 87, 80.
+struct Plan {
+  int tile = 0;  // rows; 256: wide
+  int parts = 1;
+  double us = 1e30;
+};
+
+template <class S>
+void consider(Plan *best, const GroupedArgs &a, const DeviceInfo &dev) {
+  const int64_t active = a.groups < a.rows ? a.groups : a.rows, mean = ceil_div(a.rows, active);
+  const int64_t row_tiles = ceil_div(mean, S::TILE), tiles = active * row_tiles * ceil_div(a.n, LANES * S::CTAS);
+  const int64_t stages = ceil_div(a.inner, S::STEP);
+  const double rows = (double)mean / (double)row_tiles;
+  for (int parts = 1; parts <= (S::SPLITS ? 8 : 1) && parts <= stages; ++parts) {
+    const int64_t rounds = ceil_div(tiles, resident_clusters<S>(S::CTAS == 2 ? 2 : parts, dev));
+    double stage, tile, launch;
+    if (S::CTAS == 2) {
+      stage = S::FP8 ? 0.48 : 0.095 + 0.00075 * rows > 0.155 ? 0.095 + 0.00075 * rows : 0.155;
+      tile = 1.0;
+      launch = 5.0;
+    } else {
+      stage = S::FP8 ? 0.45 + 0.0015 * rows : 0.23 + 0.0006 * rows;
+      tile = parts > 1 ? 1.6 + 0.024 * rows : 0.5;
+      launch = 3.3;
+    }
+    const double us = (double)rounds * ((double)ceil_div(stages, parts) * stage + tile) + launch;
+    if (us < best->us) *best = {S::TILE, parts, us};
+  }
+}
+
+template <bool FP8, bool MN>
+cudaError_t launch_best(const GroupedArgs &a, const Operands &from, const Product &p, const DeviceInfo &dev, cudaStream_t s) {
+  Plan plan;
+  consider<Config<2, 256, FP8, MN, false>>(&plan, a, dev);
+  consider<Config<1, 64, FP8, MN, false>>(&plan, a, dev);
+  if constexpr (!FP8) consider<Config<1, 128, FP8, MN, false>>(&plan, a, dev);
+  if (plan.tile == 256) return launch_rows<2, 256, FP8, MN>(a, from, p, 1, dev, s);
+  if constexpr (!FP8)
+    if (plan.tile == 128) return launch_rows<1, 128, FP8, MN>(a, from, p, plan.parts, dev, s);
+  return launch_rows<1, 64, FP8, MN>(a, from, p, plan.parts, dev, s);
+}
 
 }  // namespace
 
@@ -1181,17 +1253,8 @@ cudaError_t launch_grouped_rows_tcgen05(const GroupedArgs &a, int *status_flag, 
   p.scale_j = (int)(a.transpose_b ? kb : 1);
   p.scale_group = kb * nb;
   p.status = status_flag;
-  const int64_t active = a.groups < a.rows ? a.groups : a.rows;
-  const bool narrow = a.rows <= NARROW_ROWS * active, mn = !a.transpose_b;
-  int parts = 1;
-  if (narrow) {
-    const int64_t tiles = active * ceil_div(a.n, LANES), steps = ceil_div(a.inner, fp8 ? 128 : 64);
-    while (parts < 8 && tiles * parts * 2 <= dev.sm_count && steps >= parts * 4) parts *= 2;
-  }
-  if (narrow && fp8) e = mn ? launch_rows<1, 64, true, true>(a, from, p, parts, dev, s) : launch_rows<1, 64, true, false>(a, from, p, parts, dev, s);
-  else if (narrow) e = mn ? launch_rows<1, 64, false, true>(a, from, p, parts, dev, s) : launch_rows<1, 64, false, false>(a, from, p, parts, dev, s);
-  else if (fp8) e = mn ? launch_rows<2, 256, true, true>(a, from, p, 1, dev, s) : launch_rows<2, 256, true, false>(a, from, p, 1, dev, s);
-  else e = mn ? launch_rows<2, 256, false, true>(a, from, p, 1, dev, s) : launch_rows<2, 256, false, false>(a, from, p, 1, dev, s);
+  if (fp8) e = a.transpose_b ? launch_best<true, false>(a, from, p, dev, s) : launch_best<true, true>(a, from, p, dev, s);
+  else e = a.transpose_b ? launch_best<false, false>(a, from, p, dev, s) : launch_best<false, true>(a, from, p, dev, s);
   return from.release(s, e);
 }
 
@@ -1218,7 +1281,7 @@ cudaError_t launch_grouped_inner_tcgen05(const GroupedInnerArgs &a, int *status_
   p.status = status_flag;
   p.instruction = instruction_descriptor(a.type, a.type, true, true, LANES * 2);
   const int64_t tiles = a.groups * ceil_div(a.i_size, S::TILE) * ceil_div(a.j_size, LANES * 2);
-  return from.release(s, launch<S>(map_l, map_t, p, tiles, 1, dev.sm_count, s));
+  return from.release(s, launch<S>(map_l, map_t, p, tiles, 1, dev, s));
 }
 
 }  // namespace swb
