@@ -74,6 +74,7 @@ struct Config {
   static constexpr int TABLE = (int)kMaxGroups * 16 + 16;             // GroupTiles, and first tiles
   static constexpr int STAGES = (232448 - 1024 - 512 - PARTIAL - SCALES - STAGED - TABLE) / STAGE;
   static constexpr int SMEM = 1024 + STAGES * STAGE + PARTIAL + SCALES + STAGED + TABLE;
+  static constexpr int MOST_SORTED = CTAS == 2 ? 128 : 1;             // groups
   static constexpr int ROUND = 16 * CTAS;                             // N of an MMA is a multiple of this
 };
 
@@ -100,6 +101,7 @@ struct Product {
   uint32_t instruction;           // descriptor without N
   bool half_out;
   const float *a_scales, *b_scales;
+  bool sorted;                    // groups are taken by the work of a tile, largest first, and the walkers to and fro
   int col_tiles;                  // tiles along the columns
   Divisor per_band;               // tiles of eight row tiles
   Divisor per_group, per_column;  // inner form: tiles of a group, of a column of tiles
@@ -308,8 +310,15 @@ __device__ __forceinline__ Tile uniform(const Tile &t) {  // the same in all lan
 template <class S>
 struct Tiles {
   const GroupTiles *spans;
-  const int *first;  // first tile of each group, and the end
-  int groups, total;
+  const int *first;       // first tile of each group, in the order in which they are taken, and the end
+  const uint16_t *order;  // NULL: as they come
+  int groups, total, walker, walkers;
+
+  // The tile of this walker (CTA, pair, cluster) in a round; there may be none in the last.
+  __device__ __forceinline__ int of_round(int round) const {
+    return round * walkers + (order && round % 2 == 1 ? walkers - 1 - walker : walker);
+  }
+  __device__ __forceinline__ int rounds() const { return (total + walkers - 1) / walkers; }
 
   __device__ __forceinline__ Tile at(int t, const Product &p, int part, int parts) const {
     Tile tile;
@@ -317,6 +326,7 @@ struct Tiles {
       static_assert(S::TILE == LANES * S::CTAS, "");  // square tiles
       int local, it;
       tile.group = p.per_group.divide(t, &local);
+      if (order) tile.group = order[tile.group];
       tile.col0 = p.per_column.divide(local, &it) * (LANES * S::CTAS);
       tile.row0 = it * S::TILE;
       tile.valid = p.inner - tile.row0 < S::TILE ? p.inner - tile.row0 : S::TILE;
@@ -333,8 +343,8 @@ struct Tiles {
         const int mid = (lo + hi) / 2;
         if (first[mid] <= t) lo = mid; else hi = mid;
       }
-      tile.group = lo;
-      const GroupTiles span = spans[lo];
+      tile.group = order ? order[lo] : lo;
+      const GroupTiles span = spans[tile.group];
       // bands of eight row tiles, column tile after column tile within one: what runs at a time shares both operands in L2
       int in_band, in_rows;
       const int band = p.per_band.divide(t - first[lo], &in_band);
@@ -361,6 +371,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[S::STAGES], bar_empty[S::STAGES], bar_landed[S::STAGES];
   __shared__ __align__(8) uint64_t bar_sums[S::BUFFERS], bar_stored[S::BUFFERS], bar_parts, bar_added;
+  __shared__ uint16_t order[S::MOST_SORTED];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
 
@@ -374,7 +385,6 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   int *first = reinterpret_cast<int *>(spans + kMaxGroups);
   const int rank = S::CTAS == 2 || S::SPLITS ? (int)(blockIdx.x % (unsigned)(S::CTAS == 2 ? 2 : parts)) : 0;
   const int part = S::CTAS == 2 ? 0 : rank;  // of the inner axis
-  const int walkers = (int)gridDim.x / (S::CTAS == 2 ? 2 : parts), walker = (int)blockIdx.x / (S::CTAS == 2 ? 2 : parts);
 
   after_previous_kernel();
   if (tid == 0) {
@@ -408,14 +418,31 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   Tiles<S> tiles;
   tiles.spans = spans;
   tiles.first = first;
+  tiles.order = S::CTAS == 2 && p.sorted ? order : nullptr;
   tiles.groups = p.groups;
+  tiles.walkers = (int)gridDim.x / (S::CTAS == 2 ? 2 : parts);
+  tiles.walker = (int)blockIdx.x / (S::CTAS == 2 ? 2 : parts);
   for (int g = tid; g < p.groups; g += S::THREADS) spans[g] = GroupTiles::of<S>(group_rows(p.offsets, g, p.rows));
   __syncthreads();
+  if (S::CTAS == 2 && p.sorted) {  // by a tile's stages (inner form) or rows, equal ones as they come
+    auto work = [&](int g) { return S::INNER ? spans[g].end - spans[g].begin : spans[g].height(); };
+    for (int g = tid; g < p.groups; g += S::THREADS) {
+      const int own = work(g);
+      int place = 0;
+      for (int h = 0; h < p.groups; ++h) {
+        const int other = work(h);
+        place += other > own || (other == own && h < g);
+      }
+      order[place] = (uint16_t)g;
+    }
+    __syncthreads();
+  }
   if constexpr (!S::INNER) {
     if (warp == 0) {
       int before = 0;
       for (int g0 = 0; g0 < p.groups; g0 += 32) {
-        int through = g0 + lane < p.groups ? spans[g0 + lane].count() * p.col_tiles : 0;
+        int through = 0;
+        if (g0 + lane < p.groups) through = spans[tiles.order ? order[g0 + lane] : g0 + lane].count() * p.col_tiles;
         const int own = through;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -438,6 +465,8 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   const uint32_t tmem = __shfl_sync(FULL, tmem_slot, 0);
   tiles.total = S::INNER ? p.groups * (int)p.per_group.d : __shfl_sync(FULL, first[p.groups], 0);
 
+  const int rounds = __shfl_sync(FULL, tiles.rounds(), 0);
+
   auto gave_up = [&] {
     failed = 1;
     atomicExch(p.status, 1);
@@ -455,7 +484,9 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
       bool ok = true;
       const bool issues = elected();
       const uint32_t leader_full = S::CTAS == 2 ? mapped(smem_u32(bar_full), 0) : smem_u32(bar_full);
-      for (int t = walker; ok && t < tiles.total; t += walkers) {
+      for (int turn = 0; ok && turn < rounds; ++turn) {
+        const int t = tiles.of_round(turn);
+        if (t >= tiles.total) continue;
         const Tile tile = uniform(tiles.at(t, p, part, parts));
         const int mine = tile.n / S::CTAS, row = tile.row0 + (S::CTAS == 2 ? rank * mine : 0);
         const int col = tile.col0 + (S::CTAS == 2 ? rank * LANES : 0);
@@ -520,7 +551,9 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
         uint32_t round = 0, made = 0;  // accumulators begun
         bool ok = true;
         const bool issues = elected();
-        for (int t = walker; ok && t < tiles.total; t += walkers) {
+        for (int turn = 0; ok && turn < rounds; ++turn) {
+          const int t = tiles.of_round(turn);
+          if (t >= tiles.total) continue;
           const Tile tile = uniform(tiles.at(t, p, part, parts));
           const uint32_t instruction = p.instruction | ((uint32_t)(tile.n >> 3) << 17);
           uint32_t sums = 0;
@@ -566,7 +599,9 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
         uint32_t used = 0, turns = 0;  // stages copied so far; a bit per stage: parity of its turns here
         bool ok = true;
         const uint32_t leader_full = S::CTAS == 2 ? mapped(smem_u32(bar_full), 0) : smem_u32(bar_full);
-        for (int t = walker; ok && t < tiles.total; t += walkers) {
+        for (int turn = 0; ok && turn < rounds; ++turn) {
+          const int t = tiles.of_round(turn);
+          if (t >= tiles.total) continue;
           const Tile tile = tiles.at(t, p, part, parts);
           used += (uint32_t)tile.k_blocks;
           if (tile.k_blocks == 0 || tile.k_valid % S::MMA_STEP == 0) continue;
@@ -642,7 +677,9 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
           out[(int64_t)(row0 + r) * p.cols + col0 + lane] = *reinterpret_cast<const uint16_t *>(staged + place(r, lane / 8) + lane % 8 * 2);
       }
     };
-    for (int t = walker; ok && t < tiles.total; t += walkers) {
+    for (int turn = 0; ok && turn < rounds; ++turn) {
+      const int t = tiles.of_round(turn);
+      if (t >= tiles.total) continue;
       const Tile tile = tiles.at(t, p, part, parts);
       if constexpr (S::INNER) {
         const int buffer = (int)(made % S::BUFFERS);
@@ -1144,6 +1181,10 @@ cudaError_t launch(const CUtensorMap &map_l, const CUtensorMap &map_t, Product p
   }
   const int cluster = S::CTAS == 2 ? 2 : parts;
   const int64_t resident = resident_clusters<S>(cluster, dev);
+  // In the order of their work tiles are dealt more evenly (16,384 rows, 32 groups of 189 to 2426, 2048 x 1536, dA and dB over and
+  // over: 226 us as they come, 218 by work; 64 groups forward 138 and 132).
+  // The order costs each CTA some 400 clocks: where walkers take one tile or two it stays as it comes.
+  p.sorted = p.groups > 1 && p.groups <= S::MOST_SORTED && most_tiles > 2 * resident;
   LaunchShape<S> shape(most_tiles < resident ? most_tiles : resident, cluster, s);
   e = cudaLaunchKernelEx(&shape.cfg, grouped_tcgen05_kernel<S>, map_l, map_t, p, parts);
   return e != cudaSuccess ? e : cudaGetLastError();
