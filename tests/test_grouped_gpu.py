@@ -249,3 +249,109 @@ def test_the_largest_number_of_groups(ctx):
     counts = [1 if g % 3 == 0 else 0 for g in range(1024)]
     check_forward(ctx, counts, 64, 128, torch.bfloat16, True)
     check_forward(ctx, counts, 24, 12, torch.bfloat16, False)
+
+
+@pytest.mark.parametrize("groups,most", [(40, 700), (128, 300), (129, 300), (300, 90)])
+@pytest.mark.parametrize("transpose_b", [False, True])
+def test_many_ragged_groups(ctx, groups, most, transpose_b):
+    """More tiles than run at a time, groups from none to many: both orders in which groups are taken."""
+    gen = torch.Generator().manual_seed(groups)
+    counts = (torch.rand(groups, generator=gen) ** 3 * most).int().tolist()
+    counts[3], counts[7] = 0, most * 2
+    check_forward(ctx, counts, 192, 520, torch.bfloat16, transpose_b, first=1, behind=3, seed=groups)
+    offsets, rows = H.offsets_of(counts, 1), sum(counts) + 2
+    A, dC = H.normal((rows, 192), torch.bfloat16, 1), H.normal((rows, 520), torch.bfloat16, 2)
+    B = H.normal((groups, 520, 192) if transpose_b else (groups, 192, 520), torch.bfloat16, 3)
+    _, dB = ctx.grouped_mm_grad(offsets, A, B, dC, transpose_b=transpose_b, need_dA=False)
+    exact, size = H.weight_gradient(offsets, A, dC, transpose_b, B)
+    H.assert_rounded_sum(dB, exact, size, max(counts))
+
+
+@pytest.mark.parametrize("rows", [3, 20, 40, 70, 100, 150, 250, 500])
+@pytest.mark.parametrize("k", [128, 192, 320, 448, 1024, 1088, 2496])
+def test_shared_inner_axes(ctx, rows, k):
+    """One group and few columns: the inner axis shared among every number of CTAs, odd ones too, by tiles of 64, 128 and 256 rows."""
+    check_forward(ctx, [rows], k, 136, torch.bfloat16, True, behind=1, seed=rows)
+    check_forward(ctx, [rows // 2, 0, rows - rows // 2], k, 40, torch.float16, False, seed=k)
+
+
+def test_subnormal_values(ctx):
+    """fp16 subnormals count as what they are, as operands and in the result."""
+    A = (torch.arange(64 * 64, device="cuda").view(64, 64) % 37).half() * 2.0 ** -24
+    B = torch.full((1, 64, 64), 2.0 ** 3, dtype=torch.float16, device="cuda")
+    C = ctx.grouped_mm(H.offsets_of([64]), A, B)
+    exact, size = H.grouped_mm(H.offsets_of([64]), A, B, False)
+    H.assert_rounded_sum(C, exact, size, 64)
+    C = ctx.grouped_mm(H.offsets_of([64]), A, B * 2.0 ** -6)
+    exact, size = H.grouped_mm(H.offsets_of([64]), A, B * 2.0 ** -6, False)
+    H.assert_rounded_sum(C, exact, size, 64)
+
+
+def test_a_value_past_the_largest(ctx):
+    """Sums above fp16's largest value become infinities, as rounding has it."""
+    A, B = torch.full((3, 64), 200.0, dtype=torch.float16, device="cuda"), torch.full((1, 64, 16), 10.0, dtype=torch.float16, device="cuda")
+    assert bool((ctx.grouped_mm(H.offsets_of([3]), A, B) == float("inf")).all())
+    assert bool((ctx.grouped_mm(H.offsets_of([3]), A.bfloat16(), B.bfloat16()) == 128000.0).all())
+
+
+def test_past_two_to_the_31_elements(ctx):
+    """Weights of 2.4e9 elements of which the last groups are used, and a result of 2.2e9."""
+    groups, k, n = 300, 1024, 7808
+    B = torch.zeros((groups, n, k), dtype=torch.bfloat16, device="cuda")
+    B[298] = H.normal((n, k), torch.bfloat16, 1)
+    A = H.normal((70, k), torch.bfloat16, 2)
+    offsets = H.offsets_of([0] * 298 + [70, 0])
+    C = ctx.grouped_mm(offsets, A, B, transpose_b=True)
+    exact, size = H.grouped_mm(H.offsets_of([70]), A, B[298:299], True)
+    H.assert_rounded_sum(C, exact, size, k)
+    del B
+    rows, n = 540000, 4096
+    A, B = H.normal((rows, 16), torch.bfloat16, 3), H.normal((2, 16, n), torch.bfloat16, 4)
+    C = ctx.grouped_mm(H.offsets_of([rows - 100, 100]), A, B)
+    exact, size = H.grouped_mm(H.offsets_of([100]), A[-100:], B[1:], False)
+    H.assert_rounded_sum(C[-100:], exact, size, 16)
+    dA, dB = ctx.grouped_mm_grad(H.offsets_of([rows - 100, 100]), A, B, C)
+    exact, size = H.grouped_mm(H.offsets_of([100]), C[-100:], B[1:], True)
+    H.assert_rounded_sum(dA[-100:], exact, size, n)
+    exact, size = H.weight_gradient(H.offsets_of([100]), A[-100:], C[-100:], False, B[1:])
+    H.assert_rounded_sum(dB[1:], exact, size, 100)
+
+
+def test_two_graphs_at_a_time(ctx):
+    """Two captured layers, whose operands off a boundary are copied in memory of their own, replayed on two streams at once."""
+    layers = []
+    for seed in range(2):
+        A, B = H.normal((300, 511), torch.bfloat16, seed), H.normal((3, 511, 333), torch.bfloat16, seed + 2)
+        offsets = H.offsets_of([100 + seed, 150, 50 - seed])
+        C = torch.empty((300, 333), dtype=torch.bfloat16, device="cuda")
+        ctx.grouped_mm(offsets, A, B, C)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ctx.grouped_mm(offsets, A, B, C)
+        layers.append((A, B, offsets, C, graph))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (A, B, offsets, C, graph), stream in zip(layers, streams):
+            with torch.cuda.stream(stream):
+                C.fill_(7.0)
+                graph.replay()
+    torch.cuda.synchronize()
+    for A, B, offsets, C, _ in layers:
+        exact, size = H.grouped_mm(offsets, A, B, False)
+        H.assert_rounded_sum(C, exact, size, 511)
+
+
+def test_other_kernels_in_between(ctx):
+    """Calls queued behind one another and behind the block-sparse product, each reading what the one before wrote."""
+    from sparsewave_b200 import workloads as W
+    m, Bb = W.config_c5(device="cuda", block_grid=160, n_rhs=128)
+    bsr = lambda: ctx.bsr_spmm("", m.block_row_ptr, m.block_col_idx, m.block_values, Bb, 16)
+    X = bsr()
+    rows = X.shape[0]
+    offsets = H.offsets_of([rows // 3, 0, rows - rows // 3])
+    W1, W2 = H.normal((3, 128, 64), torch.bfloat16, 1, 0.1), H.normal((3, 64, 128), torch.bfloat16, 2, 0.1)
+    want = ctx.grouped_mm(offsets, ctx.grouped_mm(offsets, X, W1), W2)
+    for _ in range(10):
+        got = ctx.grouped_mm(offsets, ctx.grouped_mm(offsets, bsr(), W1), W2)
+        assert torch.equal(got, want)
