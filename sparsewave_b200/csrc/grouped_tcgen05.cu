@@ -51,6 +51,7 @@ constexpr int ROW_BYTES = 128;       // of a swizzled row of an operand in share
 constexpr int BOX_BYTES = 64 * ROW_BYTES;  // a box of 64 inner rows x 64 16-bit elements
 constexpr int FIRST_STORE_WARP = 4;
 constexpr unsigned FULL = 0xffffffffu;
+constexpr int MOST_TILES = 1 << 30;  // of a call
 
 template <int CTAS_, int TILE_, bool FP8_, bool MN_, bool INNER_>
 struct Config {
@@ -439,20 +440,23 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   }
   if constexpr (!S::INNER) {
     if (warp == 0) {
-      int before = 0;
+      // In 64 bits, cut off at MOST_TILES: offsets that decrease (which no call may pass) make groups that share rows, whose tiles
+      // may be more than 32 bits count.
+      int64_t before = 0;
       for (int g0 = 0; g0 < p.groups; g0 += 32) {
-        int through = 0;
-        if (g0 + lane < p.groups) through = spans[tiles.order ? order[g0 + lane] : g0 + lane].count() * p.col_tiles;
-        const int own = through;
+        int64_t through = 0;
+        if (g0 + lane < p.groups) through = (int64_t)spans[tiles.order ? order[g0 + lane] : g0 + lane].count() * p.col_tiles;
+        const int64_t own = through;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
-          const int v = __shfl_up_sync(FULL, through, d);
+          const int64_t v = __shfl_up_sync(FULL, through, d);
           if (lane >= d) through += v;
         }
-        if (g0 + lane < p.groups) first[g0 + lane] = before + through - own;
+        const int64_t at = before + through - own;
+        if (g0 + lane < p.groups) first[g0 + lane] = (int)(at < MOST_TILES ? at : MOST_TILES);
         before += __shfl_sync(FULL, through, 31);
       }
-      if (lane == 0) first[p.groups] = before;
+      if (lane == 0) first[p.groups] = (int)(before < MOST_TILES ? before : MOST_TILES);
     }
   }
   __syncwarp();
@@ -1168,7 +1172,7 @@ template <class S>
 cudaError_t launch(const CUtensorMap &map_l, const CUtensorMap &map_t, Product p, int64_t most_tiles, int parts, const DeviceInfo &dev,
                    cudaStream_t s) {
   if (most_tiles == 0) return cudaSuccess;
-  if (most_tiles > 2147483647LL - 4096) return cudaErrorInvalidConfiguration;  // tile numbers are 32-bit
+  if (most_tiles > MOST_TILES) return cudaErrorInvalidConfiguration;
   cudaError_t e = configure<S>();
   if (e != cudaSuccess) return e;
   p.col_tiles = (int)ceil_div(p.cols, LANES * S::CTAS);

@@ -170,6 +170,44 @@ def test_wrong_offsets_touch_nothing_outside(ctx):
     assert bool((guarded[:50] == 7.0).all()) and bool((guarded[100:] == 7.0).all())
 
 
+def test_offsets_that_decrease_stay_inside(ctx):
+    """Groups that share rows make results that nobody promised, in the rows of the call alone."""
+    rows, groups = 3000, 900
+    A, B = H.normal((rows, 64), torch.bfloat16, 1), H.normal((groups, 64, 128), torch.bfloat16, 2)
+    offsets = torch.tensor([0 if g % 2 == 0 else rows for g in range(groups + 1)], dtype=torch.int32, device="cuda")
+    guarded = torch.full((rows + 200, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    ctx.grouped_mm(offsets, A, B, guarded[100:-100])
+    assert bool((guarded[:100] == 7.0).all()) and bool((guarded[-100:] == 7.0).all()) and ctx.device_status() == 0
+    _, dB = ctx.grouped_mm_grad(offsets, A, B, guarded[100:-100].contiguous(), need_dA=False)
+    exact, size = H.weight_gradient(H.offsets_of([rows]), A, guarded[100:-100], False, B[:1])
+    H.assert_rounded_sum(dB[:1], exact, size, rows)
+    assert bool((dB[1::2] == 0).all())
+
+
+@pytest.mark.parametrize("shift", [1, 2, 4, 8])
+@pytest.mark.parametrize("counts", [[5], [70, 0, 30], [400, 90]])
+def test_results_off_a_boundary(ctx, shift, counts):
+    offsets, rows = H.offsets_of(counts), sum(counts)
+    A, B = H.normal((rows, 256), torch.bfloat16, 1), H.normal((len(counts), 136, 256), torch.bfloat16, 2)
+    dC = H.normal((rows, 136), torch.bfloat16, 3)
+
+    def room(shape):
+        size = 1
+        for n in shape:
+            size *= n
+        flat = torch.full((size + 16,), 7.0, dtype=torch.bfloat16, device="cuda")
+        return flat, flat[shift:shift + size].view(shape)
+
+    flats, (C, dA, dB) = zip(*(room(s) for s in ((rows, 136), (rows, 256), tuple(B.shape))))
+    ctx.grouped_mm(offsets, A, B, C, transpose_b=True)
+    ctx.grouped_mm_grad(offsets, A, B, dC, dA, dB, transpose_b=True)
+    assert torch.equal(C, ctx.grouped_mm(offsets, A, B, transpose_b=True))
+    want = ctx.grouped_mm_grad(offsets, A, B, dC, transpose_b=True)
+    assert torch.equal(dA, want[0]) and torch.equal(dB, want[1])
+    for flat, t in zip(flats, (C, dA, dB)):
+        assert bool((flat[:shift] == 7.0).all()) and bool((flat[shift + t.numel():] == 7.0).all())
+
+
 @pytest.mark.parametrize("k,n,rows", [(512, 256, 400), (512, 256, 24), (31, 45, 70)])
 def test_captured_with_other_group_sizes(ctx, k, n, rows):
     """A captured forward and backward pass replayed with other offsets and operands, beside an eager call in between."""
