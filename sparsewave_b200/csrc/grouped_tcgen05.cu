@@ -17,7 +17,7 @@
 //
 // Operands whose rows do not lie on 16-byte boundaries, which TMA cannot copy, are first copied to rows that do, in memory from the
 // context's stream-ordered pool: of the weights those of groups with rows.  (3,001 rows, 7 groups, 1111 x 777: warps that read such
-// rows themselves and shift them into place for every tile took 62 us, the copy and the product 24.)
+// rows themselves and shift them into place for every tile took 62 us, the copy and the product 22.)
 //
 // Roles: warp 0 copies, warp 1 issues the MMAs, warp 2 clears the rows behind a group's last (inner form),
 // four warps (wide tiles: eight) from warp 4 on read the accumulators, round and store.
@@ -676,6 +676,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
             *reinterpret_cast<uint4 *>(out + (int64_t)(row0 + r) * p.cols + col0 + piece * 8) = v;
         }
       } else if (col0 + lane < p.cols) {
+        // Rows on no 16-byte boundary.  (Eight at a time 23.8 us for 21.6, pairs of columns 32: 3,001 rows, 7 groups, 1111 x 777.)
         const int count = rows_end - row0 < 32 ? rows_end - row0 : 32;
         for (int r = 0; r < count; ++r)
           out[(int64_t)(row0 + r) * p.cols + col0 + lane] = *reinterpret_cast<const uint16_t *>(staged + place(r, lane / 8) + lane % 8 * 2);
@@ -1004,55 +1005,75 @@ bool make_map(CUtensorMap *map, const void *base, int type, int64_t inner, int64
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// A matrix (or stack of them) on its way to rows on 16-byte boundaries.
-struct Realigned {
-  const uint8_t *from;
-  uint8_t *to;           // NULL: stays where it is
-  int64_t rows;          // of all matrices
-  int64_t bytes, pitch;  // of a row; of a row of the copy
-  int64_t group_rows;    // rows of a group's matrix, of which only groups with rows are copied; 0: all
-};
-
 constexpr int REALIGN_THREADS = 256, REALIGN_AHEAD = 4;
 
-// A warp copies a row, 16 bytes of the copy a lane: aligned words of the operand shifted into place.  The first and the last bytes of
-// the operand, whose words reach over it, go byte by byte.  Bytes of the copy behind a row's last are not written (copies by
-// TMA end there).
+// Matrices on their way to rows on 16-byte boundaries.
+struct Realigned {
+  const uint8_t *from;
+  uint8_t *to;
+  int matrices;          // 0: they stay where they are
+  int64_t rows;          // of a matrix
+  int64_t bytes, pitch;  // of a row; of a row of the copy
+  bool by_group;         // matrix g is copied only if group g has rows
+};
+
+// 16 bytes where `wanted`, else zeros, without a branch: loads behind branches wait for one another.
+__device__ __forceinline__ uint4 load_if(const uint8_t *p, bool wanted) {
+  uint4 v;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@q ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"(wanted ? 1 : 0));
+  return v;
+}
+// Bytes shift ... shift + 16 of two adjacent vectors.
+__device__ __forceinline__ uint4 shifted(const uint4 &low, const uint4 &high, int shift) {
+  const uint32_t w[8] = {low.x, low.y, low.z, low.w, high.x, high.y, high.z, high.w};
+  uint32_t u[7], v[5];
+#pragma unroll
+  for (int i = 0; i < 7; ++i) u[i] = shift & 4 ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) v[i] = shift & 8 ? u[i + 2] : u[i];
+  const uint32_t bits = (uint32_t)(shift & 3) * 8;
+  return make_uint4(__funnelshift_r(v[0], v[1], bits), __funnelshift_r(v[1], v[2], bits), __funnelshift_r(v[2], v[3], bits),
+                    __funnelshift_r(v[3], v[4], bits));
+}
+
+// The blocks of a y copy a matrix: first those of a, then those of b.  A warp copies a row, 16 bytes of the copy a lane: the aligned
+// vectors that hold them, shifted into place.  The first and the last bytes of the matrices, whose vectors reach over them, go byte by
+// byte.  What lies behind a row's last byte in the copy is not its own (copies by TMA end there).
 __global__ void __launch_bounds__(REALIGN_THREADS) realign_kernel(const Realigned a, const Realigned b, const int32_t *offsets, int rows) {
   after_previous_kernel();
+  const Realigned &m = (int)blockIdx.y < a.matrices ? a : b;
+  const int matrix = (int)blockIdx.y - ((int)blockIdx.y < a.matrices ? 0 : a.matrices);
+  if (m.by_group) {
+    const RowSpan span = group_rows(offsets, matrix, rows);
+    if (span.begin == span.end) return;
+  }
   const int lane = threadIdx.x % 32;
-  const int64_t first = (int64_t)blockIdx.x * (REALIGN_THREADS / 32) + threadIdx.x / 32, step = (int64_t)gridDim.x * (REALIGN_THREADS / 32);
-  for (int64_t at = first; at < a.rows + b.rows; at += step) {
-    const bool second = at >= a.rows;
-    const Realigned &m = second ? b : a;
-    const int64_t row = second ? at - a.rows : at;
-    if (!m.to) continue;
-    if (m.group_rows > 0) {
-      const RowSpan span = group_rows(offsets, (int)(row / m.group_rows), rows);
-      if (span.begin == span.end) continue;
-    }
-    const uint8_t *from = m.from + row * m.bytes, *end = m.from + m.rows * m.bytes;
-    const int shift = (int)(reinterpret_cast<uintptr_t>(from) & 3u);
+  const uint8_t *begin = m.from, *end = m.from + m.matrices * m.rows * m.bytes;
+  const int64_t pieces = (m.bytes + 15) / 16, step = (int64_t)gridDim.x * (REALIGN_THREADS / 32);
+  for (int64_t r = (int64_t)blockIdx.x * (REALIGN_THREADS / 32) + threadIdx.x / 32; r < m.rows; r += step) {
+    const int64_t row = matrix * m.rows + r;
+    const uint8_t *from = m.from + row * m.bytes;
+    const int shift = (int)(reinterpret_cast<uintptr_t>(from) & 15u);
     uint4 *to = reinterpret_cast<uint4 *>(m.to + row * m.pitch);
-    const int64_t pieces = (m.bytes + 15) / 16;
     for (int64_t q0 = lane; q0 < pieces; q0 += 32 * REALIGN_AHEAD) {
-      uint32_t w[REALIGN_AHEAD][5];
+      uint4 low[REALIGN_AHEAD], high[REALIGN_AHEAD];
 #pragma unroll
       for (int u = 0; u < REALIGN_AHEAD; ++u) {
         const uint8_t *p = from + (q0 + 32 * u) * 16 - shift;
-        const bool whole = q0 + 32 * u < pieces && p >= m.from && p + 20 <= end;
-#pragma unroll
-        for (int i = 0; i < 5; ++i) w[u][i] = whole ? __ldg(reinterpret_cast<const uint32_t *>(p) + i) : 0u;
+        const bool whole = q0 + 32 * u < pieces && p >= begin && p + 32 <= end;
+        low[u] = load_if(p, whole);
+        high[u] = load_if(p + 16, whole && shift != 0);
       }
 #pragma unroll
       for (int u = 0; u < REALIGN_AHEAD; ++u) {
         const int64_t q = q0 + 32 * u;
         const uint8_t *p = from + q * 16;
         if (q >= pieces) break;
-        if (p - shift >= m.from && p - shift + 20 <= end) {
-          const uint32_t bits = (uint32_t)shift * 8;
-          to[q] = make_uint4(__funnelshift_r(w[u][0], w[u][1], bits), __funnelshift_r(w[u][1], w[u][2], bits),
-                             __funnelshift_r(w[u][2], w[u][3], bits), __funnelshift_r(w[u][3], w[u][4], bits));
+        if (p - shift >= begin && p - shift + 32 <= end) {
+          to[q] = shift != 0 ? shifted(low[u], high[u], shift) : low[u];
         } else {
           for (int i = 0; i < 16 && q * 16 + i < m.bytes; ++i) reinterpret_cast<uint8_t *>(to + q)[i] = __ldg(p + i);
         }
@@ -1088,26 +1109,38 @@ struct Operands {
     b_pitch = b_cols;
     const bool move_a = !aligned16(a) || a_cols * size % 16 != 0, move_b = !aligned16(b) || b_cols * size % 16 != 0;
     if (!move_a && !move_b) return cudaSuccess;
-    auto padded = [&](int64_t cols) { return (cols * size + 15) / 16 * 16; };
+    auto padded = [&](int64_t cols) { return (cols * size + 127) / 128 * 128; };  // whole lines
     const int64_t b_all = (stack > 0 ? stack : 1) * b_rows;
     const int64_t a_bytes = move_a ? a_rows * padded(a_cols) : 0, b_bytes = move_b ? b_all * padded(b_cols) : 0;
     cudaError_t e = cudaMallocFromPoolAsync(&memory, (size_t)(a_bytes + b_bytes), pool, s);
     if (e != cudaSuccess) return e;
     Realigned ra = {}, rb = {};
     if (move_a) {
-      ra = {static_cast<const uint8_t *>(a_), static_cast<uint8_t *>(memory), a_rows, a_cols * size, padded(a_cols), 0};
+      ra = {static_cast<const uint8_t *>(a_), static_cast<uint8_t *>(memory), 1, a_rows, a_cols * size, padded(a_cols), false};
       a = ra.to;
       a_pitch = ra.pitch / size;
     }
     if (move_b) {
-      rb = {static_cast<const uint8_t *>(b_), static_cast<uint8_t *>(memory) + a_bytes, b_all, b_cols * size, padded(b_cols),
-            stack > 0 && offsets ? b_rows : 0};
+      rb = {static_cast<const uint8_t *>(b_), static_cast<uint8_t *>(memory) + a_bytes, (int)(stack > 0 ? stack : 1), b_rows,
+            b_cols * size, padded(b_cols), stack > 0 && offsets};
       b = rb.to;
       b_pitch = rb.pitch / size;
     }
     ++*launches;
-    const int64_t blocks = ceil_div(ra.rows + rb.rows, REALIGN_THREADS / 32), most = 8 * (int64_t)dev.sm_count;
-    e = launch_chained(realign_kernel, (unsigned)(blocks < most ? blocks : most), REALIGN_THREADS, 0, s, ra, rb, offsets, (int)rows);
+    // Blocks for a row a warp, up to 32 per SM in all, but 64 for a matrix in any case: of many groups few may have rows.
+    const int matrices = ra.matrices + rb.matrices;
+    const int64_t rows_most = ra.rows > rb.rows ? ra.rows : rb.rows, blocks = ceil_div(rows_most, REALIGN_THREADS / 32);
+    const int64_t share = 32 * (int64_t)dev.sm_count / matrices, most = share > 64 ? share : 64;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(blocks < most ? blocks : most), (unsigned)matrices);
+    cfg.blockDim = dim3(REALIGN_THREADS);
+    cfg.stream = s;
+    cfg.attrs = attribute;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, realign_kernel, ra, rb, offsets, (int)rows);
     return e != cudaSuccess ? e : cudaGetLastError();
   }
   cudaError_t release(cudaStream_t s, cudaError_t e) {
