@@ -387,7 +387,6 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   const int rank = S::CTAS == 2 || S::SPLITS ? (int)(blockIdx.x % (unsigned)(S::CTAS == 2 ? 2 : parts)) : 0;
   const int part = S::CTAS == 2 ? 0 : rank;  // of the inner axis
 
-  after_previous_kernel();
   if (tid == 0) {
     failed = 0;
     for (int s = 0; s < S::STAGES; ++s) {
@@ -405,6 +404,9 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_l) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_t) : "memory");
   }
+  after_previous_kernel();
+  GroupTiles own_span = {};  // on its way while the rest is set up
+  if (tid < p.groups) own_span = GroupTiles::of<S>(group_rows(p.offsets, tid, p.rows));
   if (warp == 1) {
     if constexpr (S::CTAS == 2) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
@@ -416,6 +418,9 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
   }
+  __syncwarp();
+  const bool in_cluster = S::CTAS == 2 || parts > 1;
+  if (in_cluster) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   Tiles<S> tiles;
   tiles.spans = spans;
   tiles.first = first;
@@ -423,7 +428,14 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   tiles.groups = p.groups;
   tiles.walkers = (int)gridDim.x / (S::CTAS == 2 ? 2 : parts);
   tiles.walker = (int)blockIdx.x / (S::CTAS == 2 ? 2 : parts);
-  for (int g = tid; g < p.groups; g += S::THREADS) spans[g] = GroupTiles::of<S>(group_rows(p.offsets, g, p.rows));
+  auto cut_off = [](int64_t tiles) { return (int)(tiles < MOST_TILES ? tiles : MOST_TILES); };
+  if (tid < p.groups) spans[tid] = own_span;
+  for (int g = tid + S::THREADS; g < p.groups; g += S::THREADS) spans[g] = GroupTiles::of<S>(group_rows(p.offsets, g, p.rows));
+  if (!S::INNER && p.groups == 1 && tid == 0) {
+    first[0] = 0;
+    first[1] = cut_off((int64_t)own_span.count() * p.col_tiles);
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (S::CTAS == 2 && p.sorted) {  // by a tile's stages (inner form) or rows, equal ones as they come
     auto work = [&](int g) { return S::INNER ? spans[g].end - spans[g].begin : spans[g].height(); };
@@ -438,7 +450,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
     }
     __syncthreads();
   }
-  if constexpr (!S::INNER) {
+  if (!S::INNER && p.groups > 1) {
     if (warp == 0) {
       // In 64 bits, cut off at MOST_TILES: offsets that decrease (which no call may pass) make groups that share rows, whose tiles
       // may be more than 32 bits count.
@@ -452,19 +464,16 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
           const int64_t v = __shfl_up_sync(FULL, through, d);
           if (lane >= d) through += v;
         }
-        const int64_t at = before + through - own;
-        if (g0 + lane < p.groups) first[g0 + lane] = (int)(at < MOST_TILES ? at : MOST_TILES);
+        if (g0 + lane < p.groups) first[g0 + lane] = cut_off(before + through - own);
         before += __shfl_sync(FULL, through, 31);
       }
-      if (lane == 0) first[p.groups] = (int)(before < MOST_TILES ? before : MOST_TILES);
+      if (lane == 0) first[p.groups] = cut_off(before);
     }
+    __syncthreads();
   }
   __syncwarp();
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  if (S::CTAS == 2 || parts > 1) {  // barriers of the other CTAs are ready too
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  }
-  __syncthreads();
+  // The barriers of the other CTAs, and the pair's TMEM, are ready too.
+  if (in_cluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = __shfl_sync(FULL, tmem_slot, 0);
   tiles.total = S::INNER ? p.groups * (int)p.per_group.d : __shfl_sync(FULL, first[p.groups], 0);
