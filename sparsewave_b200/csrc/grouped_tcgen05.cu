@@ -368,7 +368,8 @@ struct Tiles {
 template <class S>
 __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap map_l,
                                                                         const __grid_constant__ CUtensorMap map_t, const Product p,
-                                                                        const int parts) {
+                                                                        const int cluster_parts) {
+  const int parts = S::SPLITS ? cluster_parts : 1;  // CTAs that share a tile's inner axis
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[S::STAGES], bar_empty[S::STAGES], bar_landed[S::STAGES];
   __shared__ __align__(8) uint64_t bar_sums[S::BUFFERS], bar_stored[S::BUFFERS], bar_parts, bar_added;
@@ -428,10 +429,11 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   tiles.groups = p.groups;
   tiles.walkers = (int)gridDim.x / (S::CTAS == 2 ? 2 : parts);
   tiles.walker = (int)blockIdx.x / (S::CTAS == 2 ? 2 : parts);
+  const bool one_group = S::CTAS == 1 && p.groups == 1;  // (pairs: the case costs the 8-bit form registers that it lacks)
   auto cut_off = [](int64_t tiles) { return (int)(tiles < MOST_TILES ? tiles : MOST_TILES); };
   if (tid < p.groups) spans[tid] = own_span;
   for (int g = tid + S::THREADS; g < p.groups; g += S::THREADS) spans[g] = GroupTiles::of<S>(group_rows(p.offsets, g, p.rows));
-  if (!S::INNER && p.groups == 1 && tid == 0) {
+  if (one_group && tid == 0) {
     first[0] = 0;
     first[1] = cut_off((int64_t)own_span.count() * p.col_tiles);
   }
@@ -450,7 +452,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
     }
     __syncthreads();
   }
-  if (!S::INNER && p.groups > 1) {
+  if (!S::INNER && !one_group) {
     if (warp == 0) {
       // In 64 bits, cut off at MOST_TILES: offsets that decrease (which no call may pass) make groups that share rows, whose tiles
       // may be more than 32 bits count.
