@@ -32,6 +32,15 @@ __device__ __forceinline__ float scale_of(float amax, float largest) {
 template <bool E5M2>
 __device__ __forceinline__ float largest() { return E5M2 ? 57344.0f : 448.0f; }
 
+__device__ __forceinline__ float2 times(float2 v, float f) {  // both in one instruction
+  uint64_t a, b, r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(v.x), "f"(v.y));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(b) : "f"(f));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+  return v;
+}
+
 // Eight elements of a row as they lie in memory.
 template <typename T>
 struct Eight {
@@ -77,13 +86,10 @@ struct Eight {
       for (int i = 0; i < WORDS; ++i) m = max(m, w[i] & 0x7fffffffu);
       return m;
     } else {
-      uint32_t low = 0, high = 0;  // the halves of a word: the low one shifted up
+      uint32_t two = 0;  // two at a time
 #pragma unroll
-      for (int i = 0; i < WORDS; ++i) {
-        low = max(low, w[i] << 17);
-        high = max(high, w[i] & 0x7fff0000u);
-      }
-      const uint16_t bits = (uint16_t)(max(low >> 1, high) >> 16);
+      for (int i = 0; i < WORDS; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(two) : "r"(w[i] & 0x7fff7fffu));
+      const uint16_t bits = (uint16_t)max(two & 0xffffu, two >> 16);
       T v;
       memcpy(&v, &bits, 2);
       return __float_as_uint(to_f32(v));
@@ -104,7 +110,7 @@ struct Eight {
         memcpy(two, &w[i], 4);
         v = make_float2(to_f32(two[0]), to_f32(two[1]));
       }
-      out[i] = __nv_cvt_float2_to_fp8x2(make_float2(v.x * inverse, v.y * inverse), __NV_SATFINITE, KIND);
+      out[i] = __nv_cvt_float2_to_fp8x2(times(v, inverse), __NV_SATFINITE, KIND);
     }
     if constexpr (V == 8) {
       if (valid > 0) *reinterpret_cast<uint2 *>(q) = make_uint2(out[0] | (uint32_t)out[1] << 16, out[2] | (uint32_t)out[3] << 16);
@@ -138,21 +144,24 @@ __global__ void __launch_bounds__(ROWS_THREADS) quantize_rows_kernel(int64_t row
   Eight<T> v[ROWS_PER_GROUP];
 #pragma unroll
   for (int r = 0; r < ROWS_PER_GROUP; ++r) v[r].template load<V>(X + (row0 + r) * cols + col, row0 + r < rows ? valid : 0);
-  // Each lane divides for one of the rows, and the rows' scales are stored together.
+  // The maxima of four rows at a time: two steps in which a lane gives away half of its rows for the other lane's share of the
+  // half that it keeps, two for the one row that is left.  Lanes 4 r ... 4 r + 3 end with row r, divide for it and store its scale.
+  static_assert(ROWS_PER_GROUP == 4, "");
   const unsigned lanes = 0xffffu << (threadIdx.x & 16);
-  uint32_t mine = 0;
+  const bool back = lane & 8, odd = lane & 4;
+  uint32_t m[ROWS_PER_GROUP];
 #pragma unroll
-  for (int r = 0; r < ROWS_PER_GROUP; ++r) {
-    uint32_t m = v[r].amax();
-#pragma unroll
-    for (int d = 8; d > 0; d /= 2) m = max(m, __shfl_xor_sync(lanes, m, d));
-    if (lane % ROWS_PER_GROUP == r) mine = m;
-  }
+  for (int r = 0; r < ROWS_PER_GROUP; ++r) m[r] = v[r].amax();
+  const uint32_t a0 = max(back ? m[2] : m[0], __shfl_xor_sync(lanes, back ? m[0] : m[2], 8));
+  const uint32_t a1 = max(back ? m[3] : m[1], __shfl_xor_sync(lanes, back ? m[1] : m[3], 8));
+  uint32_t mine = max(odd ? a1 : a0, __shfl_xor_sync(lanes, odd ? a0 : a1, 4));
+  mine = max(mine, __shfl_xor_sync(lanes, mine, 2));
+  mine = max(mine, __shfl_xor_sync(lanes, mine, 1));
   const float scale = scale_of(__uint_as_float(mine), largest<E5M2>()), inverse = 1.0f / scale;
-  if (lane < ROWS_PER_GROUP && row0 + lane < rows) scales[block * rows + row0 + lane] = scale;
+  if (lane % 4 == 0 && row0 + lane / 4 < rows) scales[block * rows + row0 + lane / 4] = scale;
 #pragma unroll
   for (int r = 0; r < ROWS_PER_GROUP; ++r) {
-    const float f = __shfl_sync(lanes, inverse, r, 16);
+    const float f = __shfl_sync(lanes, inverse, 4 * r, 16);
     if (row0 + r < rows) v[r].template store<E5M2, V>(Q + (row0 + r) * cols + col, f, valid);
   }
 }
