@@ -30,6 +30,16 @@
 // 8-bit operands: the 128 products of a scale block are one chain of the tensor core in an accumulator of its own; the storing
 // warps add it, times the scales of its row and block, to f32 sums in their registers (two sums per fma.f32x2).
 //
+// What bounds it (one B200; ncu: profiles of these kernels).  Wide, 16 bits: the tensor pipe, 93 % of whose cycles are active (8192 rows,
+// 4 groups, 4096 x 4096, 530 clocks a stage of 512), at the clock that the power limit leaves: 8192^3 707 us = 1,555 TFLOP/s alone,
+// some 1,300 over and over at 1.2 GHz.  Wide, 8 bits: the round trip of an accumulator (products 512 clocks, their completion some
+// 500, reading 350, the next products' issue 250; two accumulators fill TMEM): 8192^3 469 us = 2,340 TFLOP/s alone.  Narrow: HBM, and
+// some 3 us of launch, set-up and pipeline fill (8 rows, 64 groups, 2048 x 1536 11.7 us for 50 MB; 512 rows 69 us for 406 MB).
+//
+// Tried: four operand boxes a stage issued by one lane's own code (250 us for 187), scales by way of shared memory (see above), a
+// tile's shared sums stored to where they are added instead of fetched (64 rows 7.7 -> 8.8 us, 256 rows 10.2 -> 13.0), storing warps
+// that sleep between polls (no change), results of 64 columns on their way while 32 are stored (no change).
+//
 // Every mbarrier wait is bounded: when one runs out the kernel raises the status word, frees its TMEM columns and returns.
 #include <cuda.h>
 #include <cuda_bf16.h>
