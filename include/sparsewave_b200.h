@@ -306,13 +306,13 @@ typedef enum swb_dtype {
  *   C        rows x n;  offsets: groups + 1 entries on the device.
  * `dtype` (SWB_BF16 or SWB_F16) is that of A, B and C; sums are f32, in the
  * tensor core's order (which cuts sums off where it would have to round them),
- * rounded once.  Offsets must not decrease; rows of no group (before offsets[0], from
- * offsets[groups] on) are neither read nor written, so that a batch may be
- * padded.  The offsets stay on the device and are read by the kernel: a call
- * can be captured in a CUDA graph and replayed with other group sizes.  They
- * are clipped to [0, rows], so that wrong ones make wrong rows and no access
- * outside the operands.  A group may be empty; inner == 0 makes zeros.  At
- * most 1024 groups (SWB_ERR_CAPACITY).  A row of C does not depend on the
+ * rounded once.  Offsets must not decrease; rows of no group (before
+ * offsets[0], from offsets[groups] on) are neither read nor written, so that a
+ * batch may be padded.  The offsets stay on the device and are read by the
+ * kernel: a call can be captured in a CUDA graph and replayed with other group
+ * sizes.  They are clipped to [0, rows]; where they decrease all groups count
+ * as empty.  A group may be empty; inner == 0 makes zeros.  At most 1024 groups
+ * (SWB_ERR_CAPACITY).  A row of C does not depend on the
  * values in other rows of A, whatever they hold.  Operands that, or whose rows,
  * do not start on 16-byte boundaries are first copied to rows that do, in
  * stream-ordered memory that the context keeps (as large as the operand). */

@@ -55,7 +55,7 @@
 namespace swb {
 namespace {
 
-constexpr uint32_t WAIT_LIMIT = 1u << 24;
+constexpr uint32_t WAIT_LIMIT = 1u << 22;  // polls of some 1.5 us each
 constexpr int LANES = 128;           // output columns of a CTA's tile
 constexpr int ROW_BYTES = 128;       // of a swizzled row of an operand in shared memory
 constexpr int BOX_BYTES = 64 * ROW_BYTES;  // a box of 64 inner rows x 64 16-bit elements
@@ -416,8 +416,8 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_t) : "memory");
   }
   after_previous_kernel();
-  GroupTiles own_span = {};  // on its way while the rest is set up
-  if (tid < p.groups) own_span = GroupTiles::of<S>(group_rows(p.offsets, tid, p.rows));
+  RowSpan own_rows = {};  // on its way while the rest is set up
+  if (tid < p.groups) own_rows = group_rows(p.offsets, tid, p.rows);
   if (warp == 1) {
     if constexpr (S::CTAS == 2) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
@@ -440,13 +440,13 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   tiles.walkers = (int)gridDim.x / (S::CTAS == 2 ? 2 : parts);
   tiles.walker = (int)blockIdx.x / (S::CTAS == 2 ? 2 : parts);
   const bool one_group = S::CTAS == 1 && p.groups == 1;  // (pairs: the case costs the 8-bit form registers that it lacks)
-  auto cut_off = [](int64_t tiles) { return (int)(tiles < MOST_TILES ? tiles : MOST_TILES); };
-  if (tid < p.groups) spans[tid] = own_span;
-  for (int g = tid + S::THREADS; g < p.groups; g += S::THREADS) spans[g] = GroupTiles::of<S>(group_rows(p.offsets, g, p.rows));
-  if (one_group && tid == 0) {
-    first[0] = 0;
-    first[1] = cut_off((int64_t)own_span.count() * p.col_tiles);
-  }
+  bool decreasing = own_rows.decreasing;
+  for (int g = tid + S::THREADS; g < p.groups; g += S::THREADS) decreasing |= group_rows(p.offsets, g, p.rows).decreasing;
+  if (tid == 0) first[0] = 0;
+  const bool none = __syncthreads_or(decreasing);  // groups that share rows would make work without bounds: all count as empty
+  if (tid < p.groups) spans[tid] = GroupTiles::of<S>(none ? RowSpan{0, 0} : own_rows);
+  for (int g = tid + S::THREADS; g < p.groups; g += S::THREADS)
+    spans[g] = GroupTiles::of<S>(none ? RowSpan{0, 0} : group_rows(p.offsets, g, p.rows));
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (S::CTAS == 2 && p.sorted) {  // by a tile's stages (inner form) or rows, equal ones as they come
@@ -464,22 +464,20 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   }
   if (!S::INNER && !one_group) {
     if (warp == 0) {
-      // In 64 bits, cut off at MOST_TILES: offsets that decrease (which no call may pass) make groups that share rows, whose tiles
-      // may be more than 32 bits count.
-      int64_t before = 0;
+      int before = 0;
       for (int g0 = 0; g0 < p.groups; g0 += 32) {
-        int64_t through = 0;
-        if (g0 + lane < p.groups) through = (int64_t)spans[tiles.order ? order[g0 + lane] : g0 + lane].count() * p.col_tiles;
-        const int64_t own = through;
+        int through = 0;
+        if (g0 + lane < p.groups) through = spans[tiles.order ? order[g0 + lane] : g0 + lane].count() * p.col_tiles;
+        const int own = through;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
-          const int64_t v = __shfl_up_sync(FULL, through, d);
+          const int v = __shfl_up_sync(FULL, through, d);
           if (lane >= d) through += v;
         }
-        if (g0 + lane < p.groups) first[g0 + lane] = cut_off(before + through - own);
+        if (g0 + lane < p.groups) first[g0 + lane] = before + through - own;
         before += __shfl_sync(FULL, through, 31);
       }
-      if (lane == 0) first[p.groups] = cut_off(before);
+      if (lane == 0) first[p.groups] = before;
     }
     __syncthreads();
   }
@@ -488,7 +486,8 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   if (in_cluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = __shfl_sync(FULL, tmem_slot, 0);
-  tiles.total = S::INNER ? p.groups * (int)p.per_group.d : __shfl_sync(FULL, first[p.groups], 0);
+  if constexpr (S::INNER) tiles.total = p.groups * (int)p.per_group.d;
+  else tiles.total = __shfl_sync(FULL, one_group ? spans[0].count() * p.col_tiles : first[p.groups], 0);
 
   const int rounds = __shfl_sync(FULL, tiles.rounds(), 0);
 
@@ -1106,9 +1105,12 @@ __global__ void __launch_bounds__(REALIGN_THREADS) realign_kernel(const Realigne
 // Rows of the groups as zeros, for an inner axis without elements.
 __global__ void __launch_bounds__(256) zero_rows_kernel(uint16_t *out, const int32_t *offsets, int groups, int rows, int64_t cols) {
   after_previous_kernel();
+  bool decreasing = false;
+  for (int g = threadIdx.x; g < groups; g += 256) decreasing |= group_rows(offsets, g, rows).decreasing;
+  if (__syncthreads_or(decreasing)) return;
   for (int g = 0; g < groups; ++g) {
     const RowSpan span = group_rows(offsets, g, rows);
-    for (int64_t i = span.begin * cols + blockIdx.x * 256 + threadIdx.x; i < span.end * cols; i += (int64_t)gridDim.x * 256) out[i] = 0;
+    for (int64_t i = (int64_t)span.begin * cols + blockIdx.x * 256 + threadIdx.x; i < span.end * cols; i += (int64_t)gridDim.x * 256) out[i] = 0;
   }
 }
 

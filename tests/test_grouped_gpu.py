@@ -170,18 +170,20 @@ def test_wrong_offsets_touch_nothing_outside(ctx):
     assert bool((guarded[:50] == 7.0).all()) and bool((guarded[100:] == 7.0).all())
 
 
-def test_offsets_that_decrease_stay_inside(ctx):
-    """Groups that share rows make results that nobody promised, in the rows of the call alone."""
-    rows, groups = 3000, 900
-    A, B = H.normal((rows, 64), torch.bfloat16, 1), H.normal((groups, 64, 128), torch.bfloat16, 2)
+@pytest.mark.parametrize("rows,groups,k,n", [(3000, 900, 64, 128), (40, 2, 64, 128), (3000, 12, 33, 50)])
+def test_offsets_that_decrease_make_no_rows(ctx, rows, groups, k, n):
+    A, B = H.normal((rows, k), torch.bfloat16, 1), H.normal((groups, k, n), torch.bfloat16, 2)
     offsets = torch.tensor([0 if g % 2 == 0 else rows for g in range(groups + 1)], dtype=torch.int32, device="cuda")
-    guarded = torch.full((rows + 200, 128), 7.0, dtype=torch.bfloat16, device="cuda")
-    ctx.grouped_mm(offsets, A, B, guarded[100:-100])
-    assert bool((guarded[:100] == 7.0).all()) and bool((guarded[-100:] == 7.0).all()) and ctx.device_status() == 0
-    _, dB = ctx.grouped_mm_grad(offsets, A, B, guarded[100:-100].contiguous(), need_dA=False)
-    exact, size = H.weight_gradient(H.offsets_of([rows]), A, guarded[100:-100], False, B[:1])
-    H.assert_rounded_sum(dB[:1], exact, size, rows)
-    assert bool((dB[1::2] == 0).all())
+    C, dA, dC = torch.full((rows, n), 7.0, dtype=torch.bfloat16, device="cuda"), torch.full_like(A, 7.0), H.normal((rows, n), torch.bfloat16, 3)
+    ctx.grouped_mm(offsets, A, B, C)
+    _, dB = ctx.grouped_mm_grad(offsets, A, B, dC, dA)
+    assert bool((C == 7.0).all()) and bool((dA == 7.0).all()) and bool((dB == 0).all()) and ctx.device_status() == 0
+    one = torch.tensor([5, 3], dtype=torch.int32, device="cuda")
+    ctx.grouped_mm(one, A, B[:1], C)
+    assert bool((C == 7.0).all())
+    ctx.grouped_mm(H.offsets_of([rows]), A, B[:1], C)
+    exact, size = H.grouped_mm(H.offsets_of([rows]), A, B[:1], False)
+    H.assert_rounded_sum(C, exact, size, k)
 
 
 @pytest.mark.parametrize("shift", [1, 2, 4, 8])
