@@ -360,8 +360,8 @@ SWB_API int swb_fp8_quantize_blocks(swb_context *ctx, int32_t dtype,
  *   B        inner x n, or n x inner with transpose_b, with the scales of
  *            swb_fp8_quantize_blocks on that matrix;
  *   C        rows x n, bf16.
- * a_dtype and b_dtype are SWB_E4M3 or SWB_E5M2 each.  Both the sum of a block
- * and the sum of the scaled blocks are f32.  The gradient with respect to A is
+ * a_dtype and b_dtype are SWB_E4M3 or SWB_E5M2 each.  The sum of a block, the
+ * product of its two scales and the sum of the scaled blocks are f32.  The gradient with respect to A is
  * the same call on dC quantised by rows and the same B with the other
  * transpose_b; the gradient with respect to B is swb_grouped_mm_grad's on the
  * 16-bit A and dC (8-bit A has its scales along the wrong axis). */
