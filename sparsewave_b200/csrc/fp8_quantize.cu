@@ -70,6 +70,10 @@ struct Eight {
           const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p + i * PER_WORD));
           w[i] = v.x; w[i + 1] = v.y;
         }
+    } else if constexpr (BYTES == 4 && sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i)
+        if (2 * i < valid) w[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -121,6 +125,10 @@ struct Eight {
 #pragma unroll
       for (int i = 0; i < 4; i += 2)
         if (2 * i < valid) *reinterpret_cast<uint32_t *>(q + 2 * i) = out[i] | (uint32_t)out[i + 1] << 16;
+    } else if constexpr (V == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (2 * i < valid) *reinterpret_cast<uint16_t *>(q + 2 * i) = out[i];
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -205,10 +213,10 @@ __global__ void __launch_bounds__(BLOCK_THREADS) quantize_blocks_kernel(int64_t 
   }
 }
 
-// Elements per load and store: 8 or 4 where rows of X and Q start on such a boundary, else 1.
+// Elements per load and store: 8, 4 or 2 where rows of X and Q start on such a boundary, else 1.
 template <typename T>
 int vector_width(const QuantizeArgs &a) {
-  for (int v : {8, 4}) {
+  for (int v : {8, 4, 2}) {
     const size_t bytes = sizeof(T) * v < 16 ? sizeof(T) * v : 16;
     if (a.cols % v == 0 && reinterpret_cast<uintptr_t>(a.X) % bytes == 0 && reinterpret_cast<uintptr_t>(a.Q) % v == 0) return v;
   }
@@ -240,6 +248,7 @@ cudaError_t launch_width(const QuantizeArgs &a, bool by_rows, cudaStream_t s) {
   switch (vector_width<T>(a)) {
     case 8: return launch_type<T, 8>(a, by_rows, s);
     case 4: return launch_type<T, 4>(a, by_rows, s);
+    case 2: return launch_type<T, 2>(a, by_rows, s);
   }
   return launch_type<T, 1>(a, by_rows, s);
 }

@@ -63,8 +63,10 @@ constexpr int FIRST_STORE_WARP = 4;
 constexpr unsigned FULL = 0xffffffffu;
 constexpr int MOST_TILES = 1 << 30;  // of a call
 
-template <int CTAS_, int TILE_, bool FP8_, bool MN_, bool INNER_>
+// SHARED (inner form): a group's rows are shared among p.splits parts, whose f32 sums go to p.partials.
+template <int CTAS_, int TILE_, bool FP8_, bool MN_, bool INNER_, bool SHARED_ = false>
 struct Config {
+  static constexpr bool SHARED = SHARED_;
   static constexpr int CTAS = CTAS_, TILE = TILE_;   // TILE: accumulator columns, the rows of a tile
   static constexpr bool FP8 = FP8_, MN = MN_, INNER = INNER_;  // MN: the lanes' operand has its columns contiguous
   static constexpr bool ROWS_ON_LANES = (FP8 && CTAS == 2) || INNER;  // see above
@@ -116,6 +118,9 @@ struct Product {
   int col_tiles;                  // tiles along the columns
   Divisor per_band;               // tiles of eight row tiles
   Divisor per_group, per_column;  // inner form: tiles of a group, of a column of tiles
+  Divisor splits;                 // ... and parts of its rows, whose f32 sums lie in `partials`, rows of `pitch`, where it is above 1
+  float *partials;
+  int64_t pitch;
   int scale_k, scale_j;
   int64_t scale_group;
   int *status;
@@ -343,11 +348,22 @@ struct Tiles {
       tile.valid = p.inner - tile.row0 < S::TILE ? p.inner - tile.row0 : S::TILE;
       const int n = p.cols - tile.col0 < S::TILE ? p.cols - tile.col0 : S::TILE;
       tile.n = (n + S::ROUND - 1) / S::ROUND * S::ROUND;
-      const GroupTiles span = spans[tile.group];
-      const int m = span.end - span.begin;
-      tile.k0 = span.begin;
-      tile.k_blocks = (m + S::STEP - 1) / S::STEP;
-      tile.k_valid = m - (tile.k_blocks - 1) * S::STEP;
+      if constexpr (S::SHARED) {  // a part of the group's rows
+        int sub, rest;
+        const GroupTiles span = spans[p.splits.divide(tile.group, &sub)];
+        const int blocks = (span.end - span.begin + S::STEP - 1) / S::STEP;
+        const int each = p.splits.divide(blocks + (int)p.splits.d - 1, &rest);
+        tile.k0 = span.begin + (each * sub < blocks ? each * sub : blocks) * S::STEP;
+        const int left = span.end - tile.k0 > 0 ? span.end - tile.k0 : 0, m = left < each * S::STEP ? left : each * S::STEP;
+        tile.k_blocks = (m + S::STEP - 1) / S::STEP;
+        tile.k_valid = m - (tile.k_blocks - 1) * S::STEP;
+      } else {
+        const GroupTiles span = spans[tile.group];
+        const int m = span.end - span.begin;
+        tile.k0 = span.begin;
+        tile.k_blocks = (m + S::STEP - 1) / S::STEP;
+        tile.k_valid = m - (tile.k_blocks - 1) * S::STEP;
+      }
     } else {
       int lo = 0, hi = groups;  // the last group whose first tile is at most t
       while (hi - lo > 1) {
@@ -486,7 +502,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
   if (in_cluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = __shfl_sync(FULL, tmem_slot, 0);
-  if constexpr (S::INNER) tiles.total = p.groups * (int)p.per_group.d;
+  if constexpr (S::INNER) tiles.total = p.groups * (int)((S::SHARED ? p.splits.d : 1u) * p.per_group.d);
   else tiles.total = __shfl_sync(FULL, one_group ? spans[0].count() * p.col_tiles : first[p.groups], 0);
 
   const int rounds = __shfl_sync(FULL, tiles.rounds(), 0);
@@ -678,7 +694,9 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
     // Rows of 64 bytes, whose four pieces of 16 change places from row pair to row pair: eight rows' pieces lie in different banks.
     uint8_t *staged = staged_all + store_warp * 32 * 64;
     auto place = [](int row, int piece) { return row * 64 + ((piece ^ (row >> 1 & 3)) * 16); };
-    const bool vectors = p.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
+    // Bytes on whose boundary every row of C starts, up to 16.
+    const uint32_t start = (uint32_t)p.cols * 2u | (uint32_t)reinterpret_cast<uintptr_t>(p.out);
+    const int width = start % 16 == 0 ? 16 : start % 8 == 0 ? 8 : 2;
     auto lay_down = [&](const uint32_t (&w)[16]) {  // the lane's row
       __syncwarp();
 #pragma unroll
@@ -687,7 +705,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
     };
     auto store_block = [&](uint16_t *out, int row0, int rows_end, int col0) {
       __syncwarp();
-      if (vectors) {
+      if (width == 16) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = i * 8 + lane / 4, piece = lane % 4;
@@ -695,8 +713,16 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
           if (row0 + r < rows_end && col0 + piece * 8 < p.cols)
             *reinterpret_cast<uint4 *>(out + (int64_t)(row0 + r) * p.cols + col0 + piece * 8) = v;
         }
+      } else if (width == 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = i * 4 + lane / 8, piece = lane % 8;
+          const uint2 v = *reinterpret_cast<const uint2 *>(staged + place(r, piece / 2) + piece % 2 * 8);
+          if (row0 + r < rows_end && col0 + piece * 4 < p.cols)
+            *reinterpret_cast<uint2 *>(out + (int64_t)(row0 + r) * p.cols + col0 + piece * 4) = v;
+        }
       } else if (col0 + lane < p.cols) {
-        // Rows on no 16-byte boundary.  (Eight at a time 23.8 us for 21.6, pairs of columns 32: 3,001 rows, 7 groups, 1111 x 777.)
+        // Rows on no 8-byte boundary.  (Four bytes at a time where rows allow it: no change.  Eight at a time 23.8 us for 21.6, pairs of columns 32: 3,001 rows, 7 groups, 1111 x 777.)
         const int count = rows_end - row0 < 32 ? rows_end - row0 : 32;
         for (int r = 0; r < count; ++r)
           out[(int64_t)(row0 + r) * p.cols + col0 + lane] = *reinterpret_cast<const uint16_t *>(staged + place(r, lane / 8) + lane % 8 * 2);
@@ -720,11 +746,20 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
             tmem_wait_loads();
             if (c + 32 >= c_end) release_sums(buffer);
           }
+          if constexpr (S::SHARED) {
+            const int row = tile.row0 + rank * LANES + quarter * 32 + lane;
+            float *to = p.partials + ((int64_t)tile.group * p.inner + row) * p.pitch + tile.col0 + c;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            w[i] = empty ? 0u : rounded_two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), p.half_out);
-          lay_down(w);
-          store_block(out, tile.row0 + rank * LANES + quarter * 32, tile.row0 + tile.valid, tile.col0 + c);
+            for (int i = 0; i < 32; i += 4)
+              if (row < tile.row0 + tile.valid && tile.col0 + c + i < p.pitch)
+                *reinterpret_cast<uint4 *>(to + i) = empty ? make_uint4(0, 0, 0, 0) : make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              w[i] = empty ? 0u : rounded_two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), p.half_out);
+            lay_down(w);
+            store_block(out, tile.row0 + rank * LANES + quarter * 32, tile.row0 + tile.valid, tile.col0 + c);
+          }
         }
         continue;
       }
@@ -1032,7 +1067,8 @@ struct Realigned {
   const uint8_t *from;
   uint8_t *to;
   int matrices;          // 0: they stay where they are
-  int64_t rows;          // of a matrix
+  int64_t rows;          // of a matrix; one without a stack goes in slices of `rows`, of which the last may have fewer
+  int64_t all_rows;
   int64_t bytes, pitch;  // of a row; of a row of the copy
   bool by_group;         // matrix g is copied only if group g has rows
 };
@@ -1071,10 +1107,11 @@ __global__ void __launch_bounds__(REALIGN_THREADS) realign_kernel(const Realigne
     if (span.begin == span.end) return;
   }
   const int lane = threadIdx.x % 32;
-  const uint8_t *begin = m.from, *end = m.from + m.matrices * m.rows * m.bytes;
+  const uint8_t *begin = m.from, *end = m.from + m.all_rows * m.bytes;
   const int64_t pieces = (m.bytes + 15) / 16, step = (int64_t)gridDim.x * (REALIGN_THREADS / 32);
   for (int64_t r = (int64_t)blockIdx.x * (REALIGN_THREADS / 32) + threadIdx.x / 32; r < m.rows; r += step) {
     const int64_t row = matrix * m.rows + r;
+    if (row >= m.all_rows) return;
     const uint8_t *from = m.from + row * m.bytes;
     const int shift = (int)(reinterpret_cast<uintptr_t>(from) & 15u);
     uint4 *to = reinterpret_cast<uint4 *>(m.to + row * m.pitch);
@@ -1114,6 +1151,20 @@ __global__ void __launch_bounds__(256) zero_rows_kernel(uint16_t *out, const int
   }
 }
 
+// Sums of the parts of a group's rows, in the order of the rows, rounded once.
+__global__ void __launch_bounds__(256) add_partials_kernel(const float *partials, uint16_t *out, int groups, int splits, int rows, int cols,
+                                                           int64_t pitch, bool half_out) {
+  after_previous_kernel();
+  const int64_t all = (int64_t)groups * rows * cols;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t line = i / cols, group = line / rows;
+    const float *from = partials + ((group * splits) * rows + (line - group * rows)) * pitch + (i - line * cols);
+    float sum = 0.0f;
+    for (int s = 0; s < splits; ++s) sum += __ldg(from + (int64_t)s * rows * pitch);
+    out[i] = rounded(sum, half_out);
+  }
+}
+
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Both operands as TMA can copy them: in place, or in memory of the stream-ordered pool that `release` gives back.
@@ -1133,19 +1184,22 @@ struct Operands {
     const bool move_a = !aligned16(a) || a_cols * size % 16 != 0, move_b = !aligned16(b) || b_cols * size % 16 != 0;
     if (!move_a && !move_b) return cudaSuccess;
     auto padded = [&](int64_t cols) { return (cols * size + 127) / 128 * 128; };  // whole lines
+    auto slice = [](int64_t all) { return all > 512 * 32768 ? ceil_div(all, 32768) : (int64_t)512; };
+    auto slices = [&](int64_t all) { return (int)ceil_div(all, slice(all)); };
     const int64_t b_all = (stack > 0 ? stack : 1) * b_rows;
     const int64_t a_bytes = move_a ? a_rows * padded(a_cols) : 0, b_bytes = move_b ? b_all * padded(b_cols) : 0;
     cudaError_t e = cudaMallocFromPoolAsync(&memory, (size_t)(a_bytes + b_bytes), pool, s);
     if (e != cudaSuccess) return e;
     Realigned ra = {}, rb = {};
     if (move_a) {
-      ra = {static_cast<const uint8_t *>(a_), static_cast<uint8_t *>(memory), 1, a_rows, a_cols * size, padded(a_cols), false};
+      ra = {static_cast<const uint8_t *>(a_), static_cast<uint8_t *>(memory), slices(a_rows), slice(a_rows), a_rows, a_cols * size,
+            padded(a_cols), false};
       a = ra.to;
       a_pitch = ra.pitch / size;
     }
     if (move_b) {
-      rb = {static_cast<const uint8_t *>(b_), static_cast<uint8_t *>(memory) + a_bytes, (int)(stack > 0 ? stack : 1), b_rows,
-            b_cols * size, padded(b_cols), stack > 0 && offsets};
+      rb = {static_cast<const uint8_t *>(b_), static_cast<uint8_t *>(memory) + a_bytes, stack > 0 ? (int)stack : slices(b_rows),
+            stack > 0 ? b_rows : slice(b_rows), b_all, b_cols * size, padded(b_cols), stack > 0 && offsets};
       b = rb.to;
       b_pitch = rb.pitch / size;
     }
@@ -1244,7 +1298,7 @@ cudaError_t launch(const CUtensorMap &map_l, const CUtensorMap &map_t, Product p
   // In the order of their work tiles are dealt more evenly (16,384 rows, 32 groups of 189 to 2426, 2048 x 1536, dA and dB over and
   // over: 226 us as they come, 218 by work; 64 groups forward 138 and 132).
   // The order costs each CTA some 400 clocks: where walkers take one tile or two it stays as it comes.
-  p.sorted = p.groups > 1 && p.groups <= S::MOST_SORTED && most_tiles > 2 * resident;
+  p.sorted = p.groups > 1 && p.groups <= S::MOST_SORTED && most_tiles > 2 * resident && !S::SHARED;
   LaunchShape<S> shape(most_tiles < resident ? most_tiles : resident, cluster, s);
   e = cudaLaunchKernelEx(&shape.cfg, grouped_tcgen05_kernel<S>, map_l, map_t, p, parts);
   return e != cudaSuccess ? e : cudaGetLastError();
@@ -1381,8 +1435,43 @@ cudaError_t launch_grouped_inner_tcgen05(const GroupedInnerArgs &a, int *status_
   p.half_out = a.type == kF16;
   p.status = status_flag;
   p.instruction = instruction_descriptor(a.type, a.type, true, true, LANES * 2);
-  const int64_t tiles = a.groups * ceil_div(a.i_size, S::TILE) * ceil_div(a.j_size, LANES * 2);
-  return from.release(s, launch<S>(map_l, map_t, p, tiles, 1, dev, s));
+  int64_t tiles = a.groups * ceil_div(a.i_size, S::TILE) * ceil_div(a.j_size, LANES * 2);
+  // Where there are fewer tiles than pairs of CTAs, each group's rows are shared among several, whose f32 sums a second kernel adds:
+  // as many as make rounds x (stages x 0.28 us + 1.5) plus 4 us and the sums' way through memory least (25,381 rows,
+  // 1408 x 512: 118 us for one, 46 for six).
+  const int64_t resident = resident_clusters<S>(2, dev), stages = ceil_div(ceil_div(a.rows, a.groups), S::STEP);
+  int splits = 1;
+  double best = 1e30;
+  for (int n = 1; n <= 32 && n <= stages && (n == 1 || tiles * n <= resident); ++n) {
+    const double bytes = n > 1 ? 8.0 * (double)n * (double)(a.groups * a.i_size) * (double)a.j_size : 0.0;
+    const double us = (double)ceil_div(tiles * n, resident) * ((double)ceil_div(stages, n) * 0.28 + 1.5) + (n > 1 ? 4.0 + bytes / 5e6 : 0.0);
+    if (us < best) {
+      best = us;
+      splits = n;
+    }
+  }
+  void *partials = nullptr;
+  p.splits = Divisor::of((uint32_t)splits);
+  p.pitch = ceil_div(a.j_size, 4) * 4;
+  if (splits > 1) {
+    tiles *= splits;
+    e = cudaMallocFromPoolAsync(&partials, (size_t)(a.groups * splits * a.i_size * p.pitch) * 4, pool, s);
+    if (e != cudaSuccess) return from.release(s, e);
+    p.partials = static_cast<float *>(partials);
+  }
+  e = splits > 1 ? launch<Config<2, 256, false, true, true, true>>(map_l, map_t, p, tiles, 1, dev, s)
+                 : launch<S>(map_l, map_t, p, tiles, 1, dev, s);
+  if (splits > 1) {
+    if (e == cudaSuccess) {
+      ++*launches;
+      const int64_t blocks = ceil_div(a.groups * a.i_size * a.j_size, 256), most = 16 * (int64_t)dev.sm_count;
+      e = launch_chained(add_partials_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0, s, p.partials, p.out, p.groups, splits,
+                         p.inner, p.cols, p.pitch, p.half_out);
+    }
+    const cudaError_t freed = cudaFreeAsync(partials, s);
+    if (e == cudaSuccess) e = freed;
+  }
+  return from.release(s, e);
 }
 
 }  // namespace swb

@@ -395,3 +395,20 @@ def test_other_kernels_in_between(ctx):
     for _ in range(10):
         got = ctx.grouped_mm(offsets, ctx.grouped_mm(offsets, bsr(), W1), W2)
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("counts", [[5000], [3001, 0], [64], [1900, 2500, 77], [20011]])
+@pytest.mark.parametrize("k,n", [(128, 128), (136, 520), (31, 45), (257, 1000)])
+@pytest.mark.parametrize("transpose_b", [False, True])
+def test_weight_gradients_of_long_groups(ctx, counts, k, n, transpose_b):
+    """Few tiles and many rows: a group's rows shared among several parts, whose sums are added; groups shorter than a part."""
+    dtype = torch.float16 if k % 2 else torch.bfloat16
+    offsets, rows = H.offsets_of(counts, 3), sum(counts) + 5
+    A, dC = H.normal((rows, k), dtype, 1), H.normal((rows, n), dtype, 2)
+    A[:3], dC[-2:] = float("nan"), float("inf")
+    B = H.normal((len(counts), n, k) if transpose_b else (len(counts), k, n), dtype, 3)
+    _, dB = ctx.grouped_mm_grad(offsets, A, B, dC, transpose_b=transpose_b, need_dA=False)
+    exact, size = H.weight_gradient(offsets, A, dC, transpose_b, B)
+    H.assert_rounded_sum(dB, exact, size, max(counts))
+    _, again = ctx.grouped_mm_grad(offsets, A, B, dC, transpose_b=transpose_b, need_dA=False)
+    assert torch.equal(dB, again) and ctx.device_status() == 0
