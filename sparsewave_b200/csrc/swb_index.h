@@ -24,6 +24,13 @@ inline bool grid_dim(int64_t blocks, unsigned *out) {
   return true;
 }
 
+// Rows of a slice of a long operand whose copy counts its slices along the y
+// axis of a grid: at least 512, and as many as leave at most 16,384 slices.
+// The slices of two operands, or of one and up to 1,024 matrices beside it, are
+// then below the 65,535 that the axis holds.  (Not a reference construct.)
+constexpr int64_t kMaxGridY = 65535, kMostSlices = 16384;
+SWB_HD int64_t slice_rows(int64_t all) { return all > 512 * kMostSlices ? ceil_div(all, kMostSlices) : 512; }
+
 // Balanced contiguous partition of [lower, upper) over `count` workers:
 // base = span / count, rem = span % count; worker w starts at
 // lower + w*base + min(w, rem) and takes base + (w < rem) positions

@@ -1,0 +1,31 @@
+"""Products grouped by expert at the limits of their launches."""
+import pytest
+import torch
+
+from tests import grouped_helpers as H
+
+pytestmark = pytest.mark.gpu
+
+
+def signs(shape, seed):
+    """-1, 0 and 1: every product, and every sum of fewer than 2^24 of them, is exact in f32."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(-1, 2, shape, generator=gen, device="cuda", dtype=torch.int8).bfloat16()
+
+
+@pytest.mark.parametrize("rows", [2 ** 24, 2 ** 24 + 1, 2 ** 25])
+@pytest.mark.parametrize("transpose_b", [False, True])
+def test_weight_gradient_of_many_rows_off_a_boundary(ctx, rows, transpose_b):
+    """Both operands are copied first, in slices of rows that one axis of the copy's grid counts (65,535 at most)."""
+    A, dC = signs((rows, 9), 1), signs((rows, 11), 2)
+    counts = [rows // 2, 0, rows - rows // 2]
+    B = torch.empty((3, 11, 9) if transpose_b else (3, 9, 11), dtype=torch.bfloat16, device="cuda")
+    _, dB = ctx.grouped_mm_grad(H.offsets_of(counts), A, B, dC, transpose_b=transpose_b, need_dA=False)
+    exact = torch.zeros(B.shape, dtype=torch.float64, device="cuda")
+    for g, lo, hi in ((0, 0, rows // 2), (2, rows // 2, rows)):
+        left, right = (dC, A) if transpose_b else (A, dC)
+        for at in range(lo, hi, 2 ** 22):
+            part = slice(at, min(at + 2 ** 22, hi))
+            exact[g] += left[part].double().t() @ right[part].double()
+    assert float(exact.abs().max()) < 2 ** 24 and torch.equal(dB, exact.bfloat16())
+    assert ctx.device_status() == 0
