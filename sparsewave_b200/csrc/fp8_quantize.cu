@@ -231,11 +231,10 @@ cudaError_t launch(const QuantizeArgs &a, bool by_rows, cudaStream_t s) {
   if (grid > 2147483647LL) return cudaErrorInvalidConfiguration;
   const T *X = static_cast<const T *>(a.X);
   uint8_t *Q = static_cast<uint8_t *>(a.Q);
-  cudaError_t e = by_rows ? launch_chained(quantize_rows_kernel<T, V, E5M2>, (unsigned)grid, ROWS_THREADS, 0, s, a.rows, a.cols,
-                                           col_blocks, X, Q, a.scales)
-                          : launch_chained(quantize_blocks_kernel<T, V, E5M2>, (unsigned)grid, BLOCK_THREADS, 0, s, a.rows, a.cols,
-                                           row_blocks, col_blocks, X, Q, a.scales);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  return by_rows ? launch_chained(quantize_rows_kernel<T, V, E5M2>, (unsigned)grid, ROWS_THREADS, 0, s, a.rows, a.cols, col_blocks, X, Q,
+                                  a.scales)
+                 : launch_chained(quantize_blocks_kernel<T, V, E5M2>, (unsigned)grid, BLOCK_THREADS, 0, s, a.rows, a.cols, row_blocks,
+                                  col_blocks, X, Q, a.scales);
 }
 
 template <typename T, int V>

@@ -1217,8 +1217,7 @@ struct Operands {
     cfg.stream = s;
     cfg.attrs = attribute;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, realign_kernel, ra, rb, offsets, (int)rows);
-    return e != cudaSuccess ? e : cudaGetLastError();
+    return cudaLaunchKernelEx(&cfg, realign_kernel, ra, rb, offsets, (int)rows);
   }
   cudaError_t release(cudaStream_t s, cudaError_t e) {
     const cudaError_t freed = memory ? cudaFreeAsync(memory, s) : cudaSuccess;
@@ -1300,8 +1299,7 @@ cudaError_t launch(const CUtensorMap &map_l, const CUtensorMap &map_t, Product p
   // The order costs each CTA some 400 clocks: where walkers take one tile or two it stays as it comes.
   p.sorted = p.groups > 1 && p.groups <= S::MOST_SORTED && most_tiles > 2 * resident && !S::SHARED;
   LaunchShape<S> shape(most_tiles < resident ? most_tiles : resident, cluster, s);
-  e = cudaLaunchKernelEx(&shape.cfg, grouped_tcgen05_kernel<S>, map_l, map_t, p, parts);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  return cudaLaunchKernelEx(&shape.cfg, grouped_tcgen05_kernel<S>, map_l, map_t, p, parts);
 }
 
 // kind::f16 and kind::f8f6f4: f32 sums (bits 4-5), types of A and B (bits 7-9, 10-12), MN-major A and B (bits 15, 16),
@@ -1383,9 +1381,8 @@ cudaError_t launch_grouped_rows_tcgen05(const GroupedArgs &a, int *status_flag, 
   if (a.rows == 0) return cudaSuccess;
   if (a.inner == 0) {
     ++*launches;
-    const cudaError_t e = launch_chained(zero_rows_kernel, (unsigned)dev.sm_count, 256, 0, s, static_cast<uint16_t *>(a.C), a.offsets,
-                                         (int)a.groups, (int)a.rows, a.n);
-    return e != cudaSuccess ? e : cudaGetLastError();
+    return launch_chained(zero_rows_kernel, (unsigned)dev.sm_count, 256, 0, s, static_cast<uint16_t *>(a.C), a.offsets, (int)a.groups,
+                          (int)a.rows, a.n);
   }
   const bool fp8 = a.a_scales != nullptr;
   Operands from;

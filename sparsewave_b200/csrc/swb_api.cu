@@ -95,7 +95,10 @@ void count_launch(swb_context *ctx) { ++ctx->launches; }
 
 namespace {
 
+// The error is reported here and not a second time: the runtime keeps that of a refused call until it is asked for, and the next
+// launch, this library's or another's, would take it for its own.
 int cuda_fail(swb_context *ctx, cudaError_t e, const char *what) {
+  (void)cudaGetLastError();
   return fail(ctx, SWB_ERR_CUDA, "CUDA error in %s: %s", what, cudaGetErrorString(e));
 }
 

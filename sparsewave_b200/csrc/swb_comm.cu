@@ -50,6 +50,7 @@ NcclApi &nccl() {
 int comm_fail(swb_context *ctx, int status, const char *what, const char *detail) {
   char buf[512];
   snprintf(buf, sizeof buf, "%s: %s", what, detail);
+  if (status == SWB_ERR_CUDA) (void)cudaGetLastError();  // reported here, and not to the next launch
   swb::set_context_error(ctx, buf);
   return status;
 }

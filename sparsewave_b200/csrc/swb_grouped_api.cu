@@ -24,13 +24,17 @@ int fail(swb_context *ctx, int status, const char *fmt, ...) {
 }
 
 int cuda_status(swb_context *ctx, cudaError_t e, const char *op) {
-  return e == cudaSuccess ? (int)SWB_OK : fail(ctx, SWB_ERR_CUDA, "CUDA error in %s launch: %s", op, cudaGetErrorString(e));
+  if (e == cudaSuccess) return SWB_OK;
+  (void)cudaGetLastError();  // reported here, and not to the next launch
+  return fail(ctx, SWB_ERR_CUDA, "CUDA error in %s launch: %s", op, cudaGetErrorString(e));
 }
 
 int check_context(swb_context *ctx) {
   if (!ctx) return fail(nullptr, SWB_ERR_INVALID_ARGUMENT, "context is NULL");
   const cudaError_t e = cudaSetDevice(swb::context_device(ctx));
-  return e == cudaSuccess ? (int)SWB_OK : fail(ctx, SWB_ERR_CUDA, "CUDA error in cudaSetDevice: %s", cudaGetErrorString(e));
+  if (e == cudaSuccess) return SWB_OK;
+  (void)cudaGetLastError();
+  return fail(ctx, SWB_ERR_CUDA, "CUDA error in cudaSetDevice: %s", cudaGetErrorString(e));
 }
 
 // Sizes of a product grouped by expert; 2^31 - 513 keeps the kernels' 32-bit steps past the end of an axis in range.

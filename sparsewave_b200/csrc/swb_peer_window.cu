@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(256) peer_allgather_kernel(const int4 *__restr
 int window_fail(swb_context *ctx, int status, const char *what, const char *detail) {
   char buf[512];
   snprintf(buf, sizeof buf, "%s: %s", what, detail);
+  if (status == SWB_ERR_CUDA) (void)cudaGetLastError();  // reported here, and not to the next launch
   set_context_error(ctx, buf);
   return status;
 }
