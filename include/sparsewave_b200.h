@@ -315,7 +315,9 @@ typedef enum swb_dtype {
  * (SWB_ERR_CAPACITY).  A row of C does not depend on the
  * values in other rows of A, whatever they hold.  Operands that, or whose rows,
  * do not start on 16-byte boundaries are first copied to rows that do, in
- * stream-ordered memory that the context keeps (as large as the operand). */
+ * stream-ordered memory that the context keeps: as many rows as the operand
+ * has (all groups' weights), each rounded up to 128 bytes, below 512 bytes to
+ * 32 and up to 16 bytes to 16. */
 SWB_API int swb_grouped_mm(swb_context *ctx, int32_t dtype, int64_t rows,
                            int64_t inner, int64_t n, int64_t groups,
                            const int32_t *offsets, const void *A, const void *B,

@@ -1183,23 +1183,23 @@ struct Operands {
     b_pitch = b_cols;
     const bool move_a = !aligned16(a) || a_cols * size % 16 != 0, move_b = !aligned16(b) || b_cols * size % 16 != 0;
     if (!move_a && !move_b) return cudaSuccess;
-    auto padded = [&](int64_t cols) { return (cols * size + 127) / 128 * 128; };  // whole lines
+    const int64_t a_row = copy_pitch(a_cols * size), b_row = copy_pitch(b_cols * size);
     auto slices = [](int64_t all) { return (int)ceil_div(all, slice_rows(all)); };
     static_assert(2 * kMostSlices <= kMaxGridY && kMostSlices + kMaxGroups <= kMaxGridY, "");
     const int64_t b_all = (stack > 0 ? stack : 1) * b_rows;
-    const int64_t a_bytes = move_a ? a_rows * padded(a_cols) : 0, b_bytes = move_b ? b_all * padded(b_cols) : 0;
+    const int64_t a_bytes = move_a ? ceil_div(a_rows * a_row, 128) * 128 : 0, b_bytes = move_b ? b_all * b_row : 0;
     cudaError_t e = cudaMallocFromPoolAsync(&memory, (size_t)(a_bytes + b_bytes), pool, s);
     if (e != cudaSuccess) return e;
     Realigned ra = {}, rb = {};
     if (move_a) {
       ra = {static_cast<const uint8_t *>(a_), static_cast<uint8_t *>(memory), slices(a_rows), slice_rows(a_rows), a_rows, a_cols * size,
-            padded(a_cols), false};
+            a_row, false};
       a = ra.to;
       a_pitch = ra.pitch / size;
     }
     if (move_b) {
       rb = {static_cast<const uint8_t *>(b_), static_cast<uint8_t *>(memory) + a_bytes, stack > 0 ? (int)stack : slices(b_rows),
-            stack > 0 ? b_rows : slice_rows(b_rows), b_all, b_cols * size, padded(b_cols), stack > 0 && offsets};
+            stack > 0 ? b_rows : slice_rows(b_rows), b_all, b_cols * size, b_row, stack > 0 && offsets};
       b = rb.to;
       b_pitch = rb.pitch / size;
     }

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from sparsewave_b200 import Context
 from tests import grouped_helpers as H
 
 pytestmark = pytest.mark.gpu
@@ -29,3 +30,19 @@ def test_weight_gradient_of_many_rows_off_a_boundary(ctx, rows, transpose_b):
             exact[g] += left[part].double().t() @ right[part].double()
     assert float(exact.abs().max()) < 2 ** 24 and torch.equal(dB, exact.bfloat16())
     assert ctx.device_status() == 0
+
+
+@pytest.mark.parametrize("k,pitch", [(1, 16), (9, 32), (100, 224), (300, 640)])
+def test_memory_of_copies(k, pitch):
+    """A call whose rows are short takes memory for them and not for whole lines (32 MB at a time, as the driver gives it out)."""
+    rows = 2 ** 21
+    A, B = signs((rows, k), 1), signs((1, k, 8), 2)
+    offsets, C = H.offsets_of([rows]), torch.empty((rows, 8), dtype=torch.bfloat16, device="cuda")
+    with Context(0) as fresh:
+        fresh.grouped_mm(H.offsets_of([8]), A[:8, :1].repeat(1, 8), B[:, :1].repeat(1, 8, 1))  # loads the kernels
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        fresh.grouped_mm(offsets, A, B, C)
+        torch.cuda.synchronize()
+        assert before - torch.cuda.mem_get_info()[0] <= rows * pitch + 2 ** 26
+    assert torch.equal(C, (A.double() @ B[0].double()).bfloat16())
