@@ -143,6 +143,13 @@ SWB_API const char *swb_version(void);
 /* Number of kernels this context has launched since creation. */
 SWB_API int64_t swb_kernel_launch_count(const swb_context *ctx);
 
+/* Gives the stream-ordered memory that the context keeps (copies of operands,
+ * partial sums: see swb_grouped_mm) back to the device, as far as the work
+ * that used it has completed; synchronise first for all of it.  Later calls
+ * take memory anew.  Captured graphs have memory of their own, which this
+ * does not touch. */
+SWB_API int swb_trim(swb_context *ctx);
+
 /* Reads the context's device status word after the work queued on `stream`
  * has finished (synchronises that stream).  0 means no kernel gave up one of
  * its bounded waits; non-zero means a tensor-core BSR kernel abandoned a wait

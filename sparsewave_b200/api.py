@@ -124,6 +124,11 @@ class Context:
     def kernel_launches(self) -> int:
         return int(self._lib.swb_kernel_launch_count(self._ctx))
 
+    def trim(self) -> None:
+        """Gives memory that the context keeps for copies of operands (see `grouped_mm`) back to the device, as far as the
+        work that used it has completed."""
+        self._check(self._lib.swb_trim(self._ctx))
+
     def device_status(self) -> int:
         """Status word of kernels with bounded waits (synchronises the current stream); 0 = healthy."""
         v = C.c_int32(-1)

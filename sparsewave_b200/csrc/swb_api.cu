@@ -265,6 +265,13 @@ int swb_create(swb_context **out_ctx, int device_ordinal) {
   return SWB_OK;
 }
 
+int swb_trim(swb_context *ctx) {
+  int st = check_ctx(ctx);
+  if (st != SWB_OK) return st;
+  SWB_CUDA(ctx, cudaMemPoolTrimTo(ctx->pool, 0));
+  return SWB_OK;
+}
+
 int swb_device_status(swb_context *ctx, swb_stream stream, int32_t *status) {
   int st = check_ctx(ctx);
   if (st != SWB_OK) return st;

@@ -5,6 +5,7 @@ import subprocess
 
 import pytest
 
+from sparsewave_b200 import _lib
 from sparsewave_b200.build import CSRC
 
 PROGRAM = r"""
@@ -51,3 +52,8 @@ def test_copied_rows_are_little_longer(numbers):
     for row, (_, _, pitch) in numbers([*range(1, 2100), 2 ** 32 - 1026]):
         assert pitch % 16 == 0 and row <= pitch < row + (16 if row <= 16 else 32 if row < 512 else 128)
         assert row < 512 or pitch <= 1.25 * row
+
+
+def test_trim_wants_a_context():
+    lib = _lib.load()
+    assert lib.swb_trim(None) == _lib.SWB_ERR_INVALID_ARGUMENT and lib.swb_last_error(None) == b"context is NULL"

@@ -46,3 +46,20 @@ def test_memory_of_copies(k, pitch):
         torch.cuda.synchronize()
         assert before - torch.cuda.mem_get_info()[0] <= rows * pitch + 2 ** 26
     assert torch.equal(C, (A.double() @ B[0].double()).bfloat16())
+
+
+def test_trim_gives_memory_back():
+    rows = 2 ** 22
+    A, B = signs((rows, 33), 1), signs((1, 33, 8), 2)
+    offsets, C = H.offsets_of([rows]), torch.empty((rows, 8), dtype=torch.bfloat16, device="cuda")
+    with Context(0) as fresh:
+        fresh.trim()  # nothing kept so far
+        fresh.grouped_mm(offsets, A, B, C)
+        torch.cuda.synchronize()
+        kept = torch.cuda.mem_get_info()[0]
+        fresh.trim()
+        assert torch.cuda.mem_get_info()[0] - kept >= rows * 96
+        want = C.clone()
+        assert torch.equal(fresh.grouped_mm(offsets, A, B, C.fill_(7.0)), want)  # memory anew
+        fresh.trim()  # with the call perhaps in flight
+        assert torch.equal(fresh.grouped_mm(offsets, A, B, C.fill_(7.0)), want)
