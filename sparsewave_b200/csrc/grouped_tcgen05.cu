@@ -599,7 +599,9 @@ __global__ void __launch_bounds__(S::THREADS, 1) grouped_tcgen05_kernel(const __
           uint32_t sums = 0;
           for (int kb = 0; kb < tile.k_blocks; ++kb) {
             const bool fresh = S::FP8 || kb == 0;
-            ok = mbar_wait(smem_u32(&bar_full[s]), round & 1u);
+            // (inner form: the rows cleared in a group's last stage are plain stores, of the pair's other CTA too)
+            if (S::INNER && kb == tile.k_blocks - 1) ok = mbar_wait<true>(smem_u32(&bar_full[s]), round & 1u);
+            else ok = mbar_wait(smem_u32(&bar_full[s]), round & 1u);
             if (fresh) {
               buffer = (int)(made % S::BUFFERS);
               if (made >= S::BUFFERS) ok = ok && mbar_wait(smem_u32(&bar_stored[buffer]), (made / S::BUFFERS - 1) & 1u);
