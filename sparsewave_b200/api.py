@@ -301,7 +301,8 @@ class Context:
     def grouped_mm_grad(self, offsets, A, B, dC, dA=None, dB=None, *, transpose_b: bool = False, need_dA: bool = True,
                         need_dB: bool = True):
         """(dA, dB) of `grouped_mm` for the gradient dC of its result; None for one that is not needed.  dB is zero for a
-        group without rows; rows of dA of no group are left as they were."""
+        group without rows; rows of dA of no group are left as they were.  B may be None where dA is not needed, A where dB
+        is not."""
         return self._fast.grouped_mm_grad(self._ctx.value, self.device, offsets, A, B, dC, dA, dB, transpose_b, need_dA,
                                           need_dB)
 

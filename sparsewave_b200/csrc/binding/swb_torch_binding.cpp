@@ -357,25 +357,32 @@ PyObject *grouped_mm(PyObject *, PyObject *const *a, Py_ssize_t n) {
   });
 }
 
-// grouped_mm_grad(ctx, device, offsets, A, B, dC, dA | None, dB | None, transpose_b, need_dA, need_dB)
+// grouped_mm_grad(ctx, device, offsets, A | None, B | None, dC, dA | None, dB | None, transpose_b, need_dA, need_dB): A may be missing where
+// dB is not needed, B where dA is not
 PyObject *grouped_mm_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return guarded(n, 11, [&]() -> PyObject * {
     swb_context *ctx = context_of(a[0]);
     const int64_t device = integer(a[1]);
-    const at::Tensor &off = operand(a[2], 1, device, "offsets"), &A = operand(a[3], 2, device, "A"),
-                     &B = operand(a[4], 3, device, "B"), &dC = operand(a[5], 2, device, "dC");
     const bool tb = truth(a[8]), need_a = truth(a[9]), need_b = truth(a[10]);
-    const int64_t rows = A.size(0), inner = A.size(1), groups = B.size(0), cols = dC.size(1);
-    const at::ScalarType dt = A.scalar_type();
+    const bool have_B = need_a || a[4] != Py_None, have_A = need_b || !have_B || a[3] != Py_None;
+    const at::Tensor &off = operand(a[2], 1, device, "offsets");
+    const at::Tensor *A = have_A ? &operand(a[3], 2, device, "A") : nullptr, *B = have_B ? &operand(a[4], 3, device, "B") : nullptr;
+    const at::Tensor &dC = operand(a[5], 2, device, "dC");
+    if (off.size(0) < 2) raise_shape("offsets must have at least 2 entries, but got " + std::to_string(off.size(0)));
+    const int64_t rows = A ? A->size(0) : dC.size(0), cols = dC.size(1), inner = A ? A->size(1) : B->size(tb ? 2 : 1);
+    const int64_t groups = B ? B->size(0) : off.size(0) - 1;
+    const at::ScalarType dt = A ? A->scalar_type() : dC.scalar_type();
     require_sizes(off, {groups + 1}, "offsets");
     require_sizes(dC, {rows, cols}, "dC");
-    require_sizes(B, {groups, tb ? cols : inner, tb ? inner : cols}, "B");
-    const int type = type_code(A, "A", Types::k16Bits);
+    const std::vector<int64_t> a_sizes{rows, inner}, b_sizes{groups, tb ? cols : inner, tb ? inner : cols};
+    if (B) require_sizes(*B, b_sizes, "B");
+    const int type = A ? type_code(*A, "A", Types::k16Bits) : type_code(dC, "dC", Types::k16Bits);
     auto *p_off = (const int32_t *)device_pointer(off, at::kInt, "offsets");
-    void *p_A = device_pointer(A, dt, "A"), *p_B = device_pointer(B, dt, "B"), *p_dC = device_pointer(dC, dt, "dC");
+    void *p_A = A ? device_pointer(*A, dt, "A") : nullptr, *p_B = B ? device_pointer(*B, dt, "B") : nullptr;
+    void *p_dC = device_pointer(dC, dt, "dC");
     at::Tensor dA, dB;
-    if (need_a) dA = output_of(a[6], A.sizes(), dt, A, device, "dA");
-    if (need_b) dB = output_of(a[7], B.sizes(), dt, A, device, "dB");
+    if (need_a) dA = output_of(a[6], a_sizes, dt, dC, device, "dA");
+    if (need_b) dB = output_of(a[7], b_sizes, dt, dC, device, "dB");
     void *p_dA = need_a ? dA.data_ptr() : nullptr, *p_dB = need_b ? dB.data_ptr() : nullptr, *s = stream_of(a[1]);
     call_library(ctx, [&] {
       return swb_grouped_mm_grad(ctx, type, rows, inner, cols, groups, p_off, p_A, p_B, p_dC, tb, p_dA, p_dB, s);
