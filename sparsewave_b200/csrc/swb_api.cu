@@ -244,22 +244,30 @@ int swb_create(swb_context **out_ctx, int device_ordinal) {
   cudaDeviceGetAttribute(&ctx->dev.sm_count, cudaDevAttrMultiProcessorCount, device_ordinal);
   cudaDeviceGetAttribute(&ctx->dev.max_smem_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, device_ordinal);
   // Status word of kernels with bounded waits (0 = no wait ever gave up).
+  const char *step = "cudaMalloc(status)";
   e = cudaMalloc(&ctx->status_flag, sizeof(int));
-  if (e == cudaSuccess) e = cudaMemset(ctx->status_flag, 0, sizeof(int));
+  if (e == cudaSuccess) {
+    step = "cudaMemset(status)";
+    e = cudaMemset(ctx->status_flag, 0, sizeof(int));
+  }
   if (e == cudaSuccess) {
     cudaMemPoolProps props = {};
     props.allocType = cudaMemAllocationTypePinned;
     props.location.type = cudaMemLocationTypeDevice;
     props.location.id = device_ordinal;
+    step = "cudaMemPoolCreate";
     e = cudaMemPoolCreate(&ctx->pool, &props);
+  }
+  if (e == cudaSuccess) {
     uint64_t keep = UINT64_MAX;
-    if (e == cudaSuccess) e = cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &keep);
+    step = "cudaMemPoolSetAttribute";
+    e = cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &keep);
   }
   if (e != cudaSuccess) {
     if (ctx->status_flag) cudaFree(ctx->status_flag);
     if (ctx->pool) cudaMemPoolDestroy(ctx->pool);
     delete ctx;
-    return cuda_fail(nullptr, e, "cudaMalloc(status)");
+    return cuda_fail(nullptr, e, step);
   }
   *out_ctx = ctx;
   return SWB_OK;
