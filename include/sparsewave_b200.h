@@ -152,8 +152,10 @@ SWB_API int swb_trim(swb_context *ctx);
 
 /* Reads the context's device status word after the work queued on `stream`
  * has finished (synchronises that stream).  0 means no kernel gave up one of
- * its bounded waits; non-zero means a tensor-core BSR kernel abandoned a wait
- * on its pipeline barriers and its output is not valid. */
+ * its bounded waits; non-zero means that a tensor-core kernel (BSR products,
+ * swb_grouped_mm, swb_grouped_mm_grad, swb_fp8_mm, swb_fp8_grouped_mm)
+ * abandoned a wait on its pipeline barriers and its output is not valid.  The
+ * word stays set.  It says nothing about a call's offsets. */
 SWB_API int swb_device_status(swb_context *ctx, swb_stream stream,
                               int32_t *status);
 
@@ -314,13 +316,18 @@ typedef enum swb_dtype {
  * `dtype` (SWB_BF16 or SWB_F16) is that of A, B and C; sums are f32, in the
  * tensor core's order (which cuts sums off where it would have to round them),
  * rounded once.  Offsets must not decrease; rows of no group (before
- * offsets[0], from offsets[groups] on) are neither read nor written, so that a
- * batch may be padded.  The offsets stay on the device and are read by the
- * kernel: a call can be captured in a CUDA graph and replayed with other group
- * sizes.  They are clipped to [0, rows]; where they decrease all groups count
- * as empty.  A group may be empty; inner == 0 makes zeros.  At most 1024 groups
- * (SWB_ERR_CAPACITY).  A row of C does not depend on the
- * values in other rows of A, whatever they hold.  Operands that, or whose rows,
+ * offsets[0], from offsets[groups] on) are not written and take part in no
+ * result, whatever they hold, so that a batch may be padded; they may be read,
+ * and have to be memory that nobody writes meanwhile.  The offsets stay on the
+ * device and are read by the kernel: a call can be captured in a CUDA graph and
+ * replayed with other group sizes.  No status tells of wrong ones: they are
+ * clipped to [0, rows], and where they decrease all groups count as empty, so
+ * that no row of C is written.  A group may be empty; inner == 0 makes zeros.
+ * At most 1024 groups (SWB_ERR_CAPACITY).  A row of C does not depend on the
+ * values in other rows of A, whatever they hold.  C must not overlap an
+ * operand.  Whether the kernel came through its waits: swb_device_status.  A
+ * call that returns an error may have begun; what its outputs hold is then not
+ * defined.  Operands that, or whose rows,
  * do not start on 16-byte boundaries are first copied to rows that do, in
  * stream-ordered memory that the context keeps: as many rows as the operand
  * has (all groups' weights), each rounded up to 128 bytes, below 512 bytes to
@@ -334,6 +341,7 @@ SWB_API int swb_grouped_mm(swb_context *ctx, int32_t dtype, int64_t rows,
  *   dA[r, :] = dC[r, :] B[g]^T;  rows of no group are left as they were;
  *   dB[g] = sum over the rows r of group g of A[r, :]^T dC[r, :], in B's
  *   layout; zeros for an empty group.
+ * Offsets, padding, overlap, errors and status as for swb_grouped_mm.
  * dA or dB may be NULL: it is not computed, and what only it needs (B, A) may
  * be NULL too.  Sums are f32, rounded once, in an order that no launch
  * changes. */
@@ -370,17 +378,19 @@ SWB_API int swb_fp8_quantize_blocks(swb_context *ctx, int32_t dtype,
  *            swb_fp8_quantize_blocks on that matrix;
  *   C        rows x n, bf16.
  * a_dtype and b_dtype are SWB_E4M3 or SWB_E5M2 each.  The sum of a block, the
- * product of its two scales and the sum of the scaled blocks are f32.  The gradient with respect to A is
- * the same call on dC quantised by rows and the same B with the other
- * transpose_b; the gradient with respect to B is swb_grouped_mm_grad's on the
- * 16-bit A and dC (8-bit A has its scales along the wrong axis). */
+ * product of its two scales and the sum of the scaled blocks are f32.
+ * Whether the kernel came through its waits: swb_device_status.  The gradient
+ * with respect to A is the same call on dC quantised by rows and the same B
+ * with the other transpose_b; the gradient with respect to B is
+ * swb_grouped_mm_grad's on the 16-bit A and dC (8-bit A has its scales along
+ * the wrong axis). */
 SWB_API int swb_fp8_mm(swb_context *ctx, int32_t a_dtype, int32_t b_dtype,
                        int64_t rows, int64_t inner, int64_t n, const void *A,
                        const float *a_scales, const void *B,
                        const float *b_scales, int32_t transpose_b, uint16_t *C,
                        swb_stream stream);
-/* The same grouped by expert as in swb_grouped_mm: B and b_scales have one
- * more axis of `groups` in front. */
+/* The same grouped by expert as in swb_grouped_mm, with its rules on offsets
+ * and padding: B and b_scales have one more axis of `groups` in front. */
 SWB_API int swb_fp8_grouped_mm(swb_context *ctx, int32_t a_dtype,
                                int32_t b_dtype, int64_t rows, int64_t inner,
                                int64_t n, int64_t groups,

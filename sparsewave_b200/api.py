@@ -130,7 +130,8 @@ class Context:
         self._check(self._lib.swb_trim(self._ctx))
 
     def device_status(self) -> int:
-        """Status word of kernels with bounded waits (synchronises the current stream); 0 = healthy."""
+        """Status word of kernels with bounded waits (synchronises the current stream): 0, or not if a tensor-core kernel (BSR,
+        grouped or 8-bit products) gave up a wait, whose output is then not valid."""
         v = C.c_int32(-1)
         self._check(self._lib.swb_device_status(self._ctx, self._stream(), C.byref(v)))
         return int(v.value)
@@ -295,7 +296,8 @@ class Context:
         """C[r] = A[r] @ B[g] for offsets[g] <= r < offsets[g + 1]: the layer of experts whose rows come sorted by
         expert.  bf16 or f16; A is rows x inner, B groups x inner x n (groups x n x inner with `transpose_b`), offsets
         groups + 1 int32 on the device, which no call copies to the host.  Rows of no group are left as they were
-        (unset in a C that the call allocates)."""
+        (unset in a C that the call allocates) and take part in no result.  Offsets must not decrease: where they do, which no
+        status tells, all groups count as empty."""
         return self._fast.grouped_mm(self._ctx.value, self.device, offsets, A, B, C_out, transpose_b)
 
     def grouped_mm_grad(self, offsets, A, B, dC, dA=None, dB=None, *, transpose_b: bool = False, need_dA: bool = True,
