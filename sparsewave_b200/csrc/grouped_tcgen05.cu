@@ -17,7 +17,8 @@
 //
 // Operands whose rows do not lie on 16-byte boundaries, which TMA cannot copy, are first copied to rows that do, in memory from the
 // context's stream-ordered pool: of the weights those of groups with rows.  (3,001 rows, 7 groups, 1111 x 777: warps that read such
-// rows themselves and shift them into place for every tile took 62 us, the copy and the product 22.)
+// rows themselves and shift them into place for every tile took 62 us, the copy and the product 21.  Not measured where a group has
+// few rows, whose weights the copy moves three times: 512 rows, 64 groups, 2047 x 1536 198 us, 2048 x 1536 69.)
 //
 // Roles: warp 0 copies, warp 1 issues the MMAs, warp 2 clears the rows behind a group's last (inner form),
 // four warps (wide tiles: eight) from warp 4 on read the accumulators, round and store.
@@ -30,11 +31,14 @@
 // 8-bit operands: the 128 products of a scale block are one chain of the tensor core in an accumulator of its own; the storing
 // warps add it, times the scales of its row and block, to f32 sums in their registers (two sums per fma.f32x2).
 //
-// What bounds it (one B200; ncu: profiles of these kernels).  Wide, 16 bits: the tensor pipe, 93 % of whose cycles are active (8192 rows,
-// 4 groups, 4096 x 4096, 530 clocks a stage of 512), at the clock that the power limit leaves: 8192^3 707 us = 1,555 TFLOP/s alone,
-// some 1,300 over and over at 1.2 GHz.  Wide, 8 bits: the round trip of an accumulator (products 512 clocks, their completion some
-// 500, reading 350, the next products' issue 250; two accumulators fill TMEM): 8192^3 469 us = 2,340 TFLOP/s alone.  Narrow: HBM, and
-// some 3 us of launch, set-up and pipeline fill (8 rows, 64 groups, 2048 x 1536 11.7 us for 50 MB; 512 rows 69 us for 406 MB).
+// What bounds it (one B200; ncu: profiles of these kernels).  Wide, 16 bits, large groups: the tensor pipe, 92 % of whose cycles are
+// active (8192 rows, 4 groups, 4096 x 4096, 530 clocks a stage of 512), at the clock that the power limit leaves: 8192^3 707 us =
+// 1,555 TFLOP/s alone, some 1,300 over and over at 1.2 GHz.  Ragged groups of some 256 rows do not fill the pipe: 62 % (16,384 rows,
+// 64 groups, 2048 x 1536, with HBM at 63 %), since a tile of 128 to 192 rows brings a whole stage of weights for its share of the
+// products.  Wide, 8 bits: the round trip of an accumulator (products 512 clocks, their completion some 500, reading 350, the next
+// products' issue 250; two accumulators fill TMEM): 8192^3 469 us = 2,340 TFLOP/s alone.  Few rows: HBM, and some 3 us of launch,
+// set-up and pipeline fill (narrow: one group of 64 rows, 4096 x 4096 11.6 us for 35 MB; wide, which takes the same time as narrow
+// tiles on many groups: 8 rows on 8 of 64, 2048 x 1536 12.1 us for 50 MB, 512 rows on 64 69 us for 406 MB).
 //
 // Tried: four operand boxes a stage issued by one lane's own code (250 us for 187), scales by way of shared memory (see above), a
 // tile's shared sums stored to where they are added instead of fetched (64 rows 7.7 -> 8.8 us, 256 rows 10.2 -> 13.0), storing warps
@@ -1296,8 +1300,9 @@ cudaError_t launch(const CUtensorMap &map_l, const CUtensorMap &map_t, Product p
   }
   const int cluster = S::CTAS == 2 ? 2 : parts;
   const int64_t resident = resident_clusters<S>(cluster, dev);
-  // In the order of their work tiles are dealt more evenly (16,384 rows, 32 groups of 189 to 2426, 2048 x 1536, dA and dB over and
-  // over: 226 us as they come, 218 by work; 64 groups forward 138 and 132).
+  // In the order of their work tiles are dealt more evenly (1,999 rows, 12 groups, a third of them empty, 1032 x 520, dA and dB:
+  // 24.2 us as they come, 23.1 by work; 16,384 rows, 32 groups of 189 to 2426, 2048 x 1536, dA and dB 220.0 and 219.1; 64 groups
+  // forward 127.1 and 126.7).
   // The order costs each CTA some 400 clocks: where walkers take one tile or two it stays as it comes.
   p.sorted = p.groups > 1 && p.groups <= S::MOST_SORTED && most_tiles > 2 * resident && !S::SHARED;
   LaunchShape<S> shape(most_tiles < resident ? most_tiles : resident, cluster, s);
